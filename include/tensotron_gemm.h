@@ -53,6 +53,7 @@ typedef struct tt_handle_s* tt_handle_t;
 #define TT_ERR_DEVICE_WAIT 5   /* a bounded device-side wait ran out (see tt_check)     */
 #define TT_ERR_STATIC_LIMIT 6  /* size beyond what a *_static entry's built-in scratch holds */
 #define TT_ERR_BAD_LABEL 7     /* tt_check: a cross-entropy label was outside [0, classes)   */
+#define TT_ERR_BAD_ADAPTER 8   /* tt_check: a row's adapter index was outside [-1, adapters) */
 
 /* math modes: 0 and 3 carry the meaning of SetCuBlasMathMode
  * (src/Tensotron/TensorRuntime.cs:332-338: 0 = FP32, 3 = TF32); 4 is new. */
@@ -144,6 +145,43 @@ TT_API int tt_linear_fwd(tt_handle_t h, void* stream, const float* x, const floa
 TT_API int tt_linear_bwd(tt_handle_t h, void* stream, const float* x, const float* w, const float* y,
                   const float* dy, float* dx, float* dw, float* dbias, int M, int N, int K, int act);
 
+/* Low-rank adapters beside a Linear layer.  No counterpart in the reference: every row m of the call brings its own
+ * adapter e_m, a pair A (rank, K), B (N, rank) with a scale s, beside the one projection that all rows share:
+ *   forward    t[m] = A[e_m] x[m]        y[m] = act(w x[m] + bias + s[e_m] B[e_m] t[m])
+ *   backward   g = dy * act'(y)          dt[m] = s[e_m] B[e_m]^T g[m]
+ *              dx[m] = w^T g[m] + A[e_m]^T dt[m]
+ *              da[e] = sum of dt[m] x[m]^T, db[e] = s[e] * sum of g[m] t[m]^T over the rows of adapter e
+ *              dw = g^T x, dbias = sum of g over all rows
+ *   row_adapter  device int32 (M): e_m in [0, adapters), or -1 for a row without an adapter (t is 0 there).  NULL:
+ *            every row has adapter 0.  Any other value is never used as an index: the row counts as one without an
+ *            adapter, and tt_check reports TT_ERR_BAD_ADAPTER.
+ *   w        (N, K), or NULL: the projection's part has been computed by another call, and the adapters' part is added
+ *            to what y (forward, before the activation) or dx (backward) holds.  bias, dw and dbias must then be NULL.
+ *   t        (M, rank).  forward: optional output.  backward: what the forward call stored, or NULL: recomputed from x.
+ * In the backward call dx, dw, dbias, da and db may each be NULL (not computed); y may be NULL when act is
+ * TT_ACT_NONE; x may be NULL when neither da nor dw is asked for and t is given.  da (adapters, rank, K) and
+ * db (adapters, N, rank) are written, zero for adapters without rows; they are not accumulated.  Outputs must not
+ * overlap inputs or each other, other than by the accumulation into y or dx.
+ * The projection's products follow the handle's math mode; the adapters' are always strict FP32.  Every sum runs in an
+ * order that depends on the shapes, the row_adapter values and the SM count only (no atomics on data).
+ * M may be 0; N and K are at least 1.  Rank up to TT_LORA_MAX_RANK and up to TT_LORA_MAX_ADAPTERS adapters (TT_ERR_UNSUPPORTED beyond).  The handle workspace
+ * holds the grouping of the rows (about 4 * (M + adapters) bytes), t and dt (M * rank floats each) and, for a
+ * backward call with an activation, g (M * N floats): tt_lora_workspace bytes, TT_ERR_WORKSPACE when it is smaller. */
+#define TT_LORA_MAX_RANK 128
+#define TT_LORA_MAX_ADAPTERS 4096
+typedef struct tt_lora_desc {
+    const float* a;      /* (adapters, rank, K)                       */
+    const float* b;      /* (adapters, N, rank)                       */
+    const float* scale;  /* device float (adapters), or NULL: all one */
+    int adapters, rank;
+} tt_lora_desc;
+TT_API size_t tt_lora_workspace(int M, int N, int K, int adapters, int rank, int act, int backward);
+TT_API int tt_lora_fwd(tt_handle_t h, void* stream, const tt_lora_desc* lora, const int* row_adapter, const float* x,
+                       const float* w, const float* bias, float* y, float* t, int M, int N, int K, int act);
+TT_API int tt_lora_bwd(tt_handle_t h, void* stream, const tt_lora_desc* lora, const int* row_adapter, const float* x,
+                       const float* w, const float* y, const float* dy, const float* t, float* dx, float* dw,
+                       float* dbias, float* da, float* db, int M, int N, int K, int act);
+
 /* CrossEntropy(mean-style) forward+backward in one launch
  * (src/Tensotron/TensorOps.Losses.cs:97-108, src/Tensotron/TensorOps.Reduce.cs:122-141):
  * labels are device int32 in [0, classes); dlogits = (softmax - onehot) * scale; *loss (device
@@ -167,6 +205,19 @@ TT_API int tt_mse_loss(tt_handle_t h, void* stream, const float* input, const fl
  * synchronises.  Needs 8 KiB of the handle workspace. */
 TT_API int tt_clip_grad_norm(tt_handle_t h, void* stream, float* grads, long long n, float max_norm, float eps,
                              float* norm_out);
+
+/* GradUtils.ClipGradNorm over the gradients of a parameter list (src/Tensotron/Optimizers.cs:383-422, which walks
+ * IEnumerable<Tensor>): one norm over all `count` tensors (grads[i], sizes[i] elements; host arrays, read during the
+ * call and not retained), norm = sqrt(sum g^2), coef = clamp(max_norm / (norm + eps), 0, 1).
+ *   scale != 0   every g is multiplied by coef, unconditionally
+ *   scale == 0   the tensors are left as they are: *coef_out goes to tt_adam_step_list, which multiplies on the fly
+ *   norm_out, coef_out   optional device floats
+ * The squares are summed in double precision in an order that depends on the sizes, the tensors' alignment and the SM
+ * count only.  A NaN among the gradients makes the norm and the coefficient NaN (and so, when scaled, every
+ * gradient); an infinite one makes the coefficient 0.  A tensor may have zero elements (its pointer is then not read);
+ * an empty list has norm 0.  Pointers are 4-byte aligned.  Needs 136 KiB of the handle workspace. */
+TT_API int tt_clip_grad_norm_list(tt_handle_t h, void* stream, int count, float* const* grads, const long long* sizes,
+                                  float max_norm, float eps, int scale, float* norm_out, float* coef_out);
 
 /* Conv2d through the batched GEMM engine (src/Tensotron/TensorOps.Conv.cs:60-80: Im2Col, then
  * MatMul((1, O, K), (N, K, L)), then the broadcast bias add; K = C*kh*kw, L = Ho*Wo; symmetric
@@ -210,6 +261,16 @@ TT_API int tt_softmax_cross_entropy_static(void* stream, const float* logits, co
 TT_API int tt_adam_step(tt_handle_t h, void* stream, float* p, const float* g, float* m, float* v,
                  float* adv, long long n, float beta1, float beta2, float lr, float eps,
                  float coupled_wd, float decoupled_factor, int advance);
+
+/* tt_adam_step over a parameter list (Adam.Step of src/Tensotron/Optimizers.cs:144-193, which launches once per
+ * tensor): p[i], g[i], m[i], v[i] of sizes[i] elements (host arrays, read during the call and not retained), `adv` and
+ * the scalars as in tt_adam_step.  grad_scale: optional device float that multiplies every gradient first, the
+ * coef_out of tt_clip_grad_norm_list: the clipped step then neither writes nor re-reads the gradients.  With `advance`
+ * the step counter moves once per call, also for an empty list. */
+TT_API int tt_adam_step_list(tt_handle_t h, void* stream, int count, float* const* p, const float* const* g,
+                             float* const* m, float* const* v, const long long* sizes, float* adv,
+                             const float* grad_scale, float beta1, float beta2, float lr, float eps, float coupled_wd,
+                             float decoupled_factor, int advance);
 
 /* The whole training step of a small MLP -- forward, loss, backward, gradient-norm clip, Adam --
  * as ONE launch (a thread-block cluster; everything stays in shared memory).  It replaces the

@@ -15,10 +15,12 @@
 #include "gemm_common.h"
 #include "gemm_generic.cuh"
 #include "linear_small.cuh"
+#include "lora.h"
 #include "mlp_step.h"
 #include "peer.cuh"
 #include "sgemm_simt.cuh"
 #include "skinny.cuh"
+#include "tensor_lists.h"
 #include "tensor_map.h"
 #include "tf32_launch.h"
 
@@ -43,8 +45,8 @@ namespace {
 
 constexpr size_t DEFAULT_WORKSPACE = 256ull << 20;
 // Device words owned by the handle: word 0 = status of the bounded waits; from word 64 on, one
-// stream-K flag per CTA (zero between launches).
-constexpr int STREAMK_FLAGS_WORD = 64, HANDLE_WORDS = 1024;
+// stream-K flag per CTA (zero between launches); behind them the tickets of kernels whose last CTA finishes the job.
+constexpr int STREAMK_FLAGS_WORD = 64, GROUP_TICKET_WORD = 960, LIST_TICKET_WORD = 992, HANDLE_WORDS = 1024;
 constexpr long long TMA_MIN_FLOP_ELEMS = 1ll << 21;  // M*N*K below this -> any-stride kernel
 constexpr long long SMALL_3XTF32_MAX_ELEMS = 1ll << 28;  // M x N x K up to which 3xTF32 runs on the strict-FP32 kernels
 constexpr long long LINEAR_SMALL_MAX_ELEMS = 1ll << 21;  // M x N x K up to which a Linear backward is ONE launch (linear_small.cuh)
@@ -1222,6 +1224,180 @@ TT_API int tt_linear_bwd(tt_handle_t h, void* stream, const float* x, const floa
                            nullptr, nullptr);
 }
 
+// ---- low-rank adapters -------------------------------------------------------------------
+
+namespace {
+size_t align256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
+
+// Byte offsets of what an adapter call keeps in the handle workspace; the projection's GEMMs work behind `end`.
+struct LoraWorkspace {
+    size_t groups, t, dt, g, end;
+};
+
+LoraWorkspace lora_workspace(int M, int N, int adapters, int rank, int act, bool backward)
+{
+    LoraWorkspace w;
+    const size_t rows = align256(sizeof(float) * static_cast<size_t>(M) * rank);
+    w.groups = 0;
+    w.t = align256(lora::groups_bytes(M, adapters));
+    w.dt = w.t + rows;
+    w.g = w.dt + (backward ? rows : 0);
+    w.end = w.g + (backward && act != TT_ACT_NONE ? align256(sizeof(float) * static_cast<size_t>(M) * N) : 0);
+    return w;
+}
+
+int lora_check(tt_handle_t h, const tt_lora_desc* lora, int M, int N, int K, int act)
+{
+    if (!h) return TT_ERR_INVALID_ARG;
+    if (M < 0 || N < 1 || K < 1) return fail(h, TT_ERR_INVALID_ARG, "an adapter call needs M >= 0, N >= 1, K >= 1");
+    if (act < TT_ACT_NONE || act > TT_ACT_TANH) return fail(h, TT_ERR_INVALID_ARG, "unknown activation");
+    if (!lora || lora->adapters < 1 || lora->rank < 1) return fail(h, TT_ERR_INVALID_ARG, "an adapter call needs at least one adapter of rank 1");
+    if (lora->adapters > TT_LORA_MAX_ADAPTERS || lora->rank > TT_LORA_MAX_RANK)
+        return fail(h, TT_ERR_UNSUPPORTED, "more adapters or a higher rank than the kernels take");
+    if (!lora->a || !lora->b) return fail(h, TT_ERR_INVALID_ARG, "null device pointer");
+    if (static_cast<long long>(M) * lora->rank > 0x7fffffffll || static_cast<long long>(M) * N > 0x7fffffffll ||
+        static_cast<long long>(M) * K > 0x7fffffffll || (N + 127) / 128 > 65535 || (K + 127) / 128 > 65535)
+        return fail(h, TT_ERR_UNSUPPORTED, "more elements than int32 offsets reach");   // like every buffer of the reference
+    return TT_OK;
+}
+
+// The grouping of the rows; all pointers null (and no launch) when every row has adapter 0.
+int lora_group(tt_handle_t h, cudaStream_t st, const tt_lora_desc* lora, const int* row_adapter, int M, const LoraWorkspace& ws,
+               lora::Groups& g)
+{
+    g = lora::Groups();
+    if (!row_adapter) return TT_OK;
+    g = lora::groups_layout(h->workspace + ws.groups, M, lora->adapters);
+    const cudaError_t e = lora::launch_group(st, g, row_adapter, M, lora->adapters, h->status + GROUP_TICKET_WORD, h->status);
+    if (e != cudaSuccess) return cuda_fail(h, e, "row grouping launch");
+    h->stats.launches++;
+    return TT_OK;
+}
+}  // namespace
+
+static_assert(TT_LORA_MAX_RANK == lora::MAX_RANK && TT_LORA_MAX_ADAPTERS == lora::MAX_ADAPTERS, "header constants");
+
+TT_API size_t tt_lora_workspace(int M, int N, int K, int adapters, int rank, int act, int backward)
+{
+    if (M < 0 || N < 1 || K < 1 || adapters < 1 || rank < 1) return 0;
+    return lora_workspace(M, N, adapters, rank, act, backward != 0).end;
+}
+
+TT_API int tt_lora_fwd(tt_handle_t h, void* stream, const tt_lora_desc* lora, const int* row_adapter, const float* x,
+                       const float* w, const float* bias, float* y, float* t, int M, int N, int K, int act)
+{
+    int rc = lora_check(h, lora, M, N, K, act);
+    if (rc) return rc;
+    if (!w && bias) return fail(h, TT_ERR_INVALID_ARG, "a bias needs the projection's weight");
+    if (M > 0 && (!y || !x)) return fail(h, TT_ERR_INVALID_ARG, "null device pointer");
+    TT_BIND(h);
+    h->stats.calls++;
+    if (M == 0) return TT_OK;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const LoraWorkspace ws = lora_workspace(M, N, lora->adapters, lora->rank, act, false);
+    if (ws.end > h->workspace_bytes) return fail(h, TT_ERR_WORKSPACE, "workspace too small for the adapters");
+    const lora::Adapters ad{lora->a, lora->b, lora->scale, lora->adapters, lora->rank};
+    lora::Groups g;
+    if ((rc = lora_group(h, st, lora, row_adapter, M, ws, g))) return rc;
+    float* tt = t ? t : reinterpret_cast<float*>(h->workspace + ws.t);
+    cudaError_t e = lora::launch_shrink(st, g, ad, true, false, x, tt, M, K, h->num_sms);
+    if (e != cudaSuccess) return cuda_fail(h, e, "adapter down-projection launch");
+    h->stats.launches++;
+    if (w) {
+        GemmCall gc{x, w, y, M, N, K, K, 1, 1, K, HostBatch(), 1, Epilogue{bias, TT_ACT_NONE}};
+        gc.ws_off = ws.end;
+        if ((rc = run_gemm(h, st, gc))) return rc;
+    }
+    e = lora::launch_expand(st, g, ad, true, true, tt, y, M, N, act);
+    if (e != cudaSuccess) return cuda_fail(h, e, "adapter up-projection launch");
+    h->stats.launches++;
+    return TT_OK;
+}
+
+TT_API int tt_lora_bwd(tt_handle_t h, void* stream, const tt_lora_desc* lora, const int* row_adapter, const float* x,
+                       const float* w, const float* y, const float* dy, const float* t, float* dx, float* dw,
+                       float* dbias, float* da, float* db, int M, int N, int K, int act)
+{
+    int rc = lora_check(h, lora, M, N, K, act);
+    if (rc) return rc;
+    if (!w && (dw || dbias)) return fail(h, TT_ERR_INVALID_ARG, "the projection's gradients need its weight");
+    if (M > 0 && (!dy || (act != TT_ACT_NONE && !y))) return fail(h, TT_ERR_INVALID_ARG, "null device pointer");
+    if (M > 0 && !x && (da || dw || (db && !t))) return fail(h, TT_ERR_INVALID_ARG, "null device pointer");
+    TT_BIND(h);
+    h->stats.calls++;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const LoraWorkspace ws = lora_workspace(M, N, lora->adapters, lora->rank, act, true);
+    size_t ws_used = ws.end;
+    if (ws_used > h->workspace_bytes) return fail(h, TT_ERR_WORKSPACE, "workspace too small for the adapters");
+    cudaError_t e;
+    if (M == 0) {
+        const auto zero = [&](float* p, size_t n) { return !p || n == 0 ? cudaSuccess : cudaMemsetAsync(p, 0, sizeof(float) * n, st); };
+        const size_t ranks = static_cast<size_t>(lora->adapters) * lora->rank;
+        if ((e = zero(da, ranks * K)) != cudaSuccess || (e = zero(db, ranks * N)) != cudaSuccess ||
+            (e = zero(dw, static_cast<size_t>(N) * K)) != cudaSuccess || (e = zero(dbias, N)) != cudaSuccess)
+            return cuda_fail(h, e, "memset of the gradients");
+        return TT_OK;
+    }
+    const lora::Adapters ad{lora->a, lora->b, lora->scale, lora->adapters, lora->rank};
+    lora::Groups g;
+    if ((rc = lora_group(h, st, lora, row_adapter, M, ws, g))) return rc;
+    // g = dy * act'(y) and the bias gradient
+    const float* grad = dy;
+    if (act != TT_ACT_NONE || dbias) {
+        const int chunks = ew::colsum_chunks(M);
+        const size_t part_bytes = dbias && chunks > 1 ? align256(sizeof(float) * static_cast<size_t>(chunks) * N) : 0;
+        if (ws_used + part_bytes > h->workspace_bytes) return fail(h, TT_ERR_WORKSPACE, "workspace too small for the adapters");
+        float* gbuf = act != TT_ACT_NONE ? reinterpret_cast<float*>(h->workspace + ws.g) : nullptr;
+        float* partial = !dbias ? nullptr : chunks == 1 ? dbias : reinterpret_cast<float*>(h->workspace + ws_used);
+        const bool vec = (N % 4 == 0) && aligned16(dy) && (!act || aligned16(y));
+        const dim3 grid((N + ew::COLSUM_COLS - 1) / ew::COLSUM_COLS, chunks);
+        if (vec) ew::act_bwd_colsum_kernel<true><<<grid, 256, 0, st>>>(y, dy, gbuf, partial, M, N, act, chunks);
+        else     ew::act_bwd_colsum_kernel<false><<<grid, 256, 0, st>>>(y, dy, gbuf, partial, M, N, act, chunks);
+        h->stats.launches++;
+        if (dbias && chunks > 1) {
+            ew::colsum_finish_kernel<<<(N + 255) / 256, 256, 0, st>>>(partial, dbias, N, chunks);
+            h->stats.launches++;
+        }
+        if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(h, e, "adapter backward elementwise launch");
+        if (gbuf) grad = gbuf;
+        ws_used += part_bytes;
+    }
+    float* dt = reinterpret_cast<float*>(h->workspace + ws.dt);
+    if (dx || da) {
+        if ((e = lora::launch_shrink(st, g, ad, false, true, grad, dt, M, N, h->num_sms)) != cudaSuccess)
+            return cuda_fail(h, e, "adapter gradient launch");
+        h->stats.launches++;
+    }
+    if (db && !t) {
+        float* tt = reinterpret_cast<float*>(h->workspace + ws.t);
+        if ((e = lora::launch_shrink(st, g, ad, true, false, x, tt, M, K, h->num_sms)) != cudaSuccess)
+            return cuda_fail(h, e, "adapter down-projection launch");
+        h->stats.launches++;
+        t = tt;
+    }
+    if (da || db) {
+        if ((e = lora::launch_outer(st, g, ad, dt, x, da, grad, t, db, M, N, K, h->num_sms)) != cudaSuccess)
+            return cuda_fail(h, e, "adapter weight gradient launch");
+        h->stats.launches++;
+    }
+    if (dx) {
+        if (w) {
+            GemmCall gx{grad, w, dx, M, K, N, N, 1, K, 1, HostBatch(), 1, Epilogue{nullptr, TT_ACT_NONE}};
+            gx.ws_off = ws_used;
+            if ((rc = run_gemm(h, st, gx))) return rc;
+        }
+        if ((e = lora::launch_expand(st, g, ad, false, false, dt, dx, M, K, TT_ACT_NONE)) != cudaSuccess)
+            return cuda_fail(h, e, "adapter input gradient launch");
+        h->stats.launches++;
+    }
+    if (dw) {
+        GemmCall gw{grad, x, dw, N, K, M, 1, N, K, 1, HostBatch(), 1, Epilogue{nullptr, TT_ACT_NONE}};
+        gw.ws_off = ws_used;
+        if ((rc = run_gemm(h, st, gw))) return rc;
+    }
+    return TT_OK;
+}
+
 namespace {
 // Fills the derived sizes; false when the description is not a valid convolution.
 bool conv_shape(const tt_conv2d_desc* d, conv::Shape& s)
@@ -1244,8 +1420,6 @@ bool conv_shape(const tt_conv2d_desc* d, conv::Shape& s)
     s.Kp = (s.K + 1 + 3) & ~3;
     return true;
 }
-
-size_t align256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
 
 struct ConvWorkspace {
     size_t col, wp, dcol, end;   // byte offsets into the handle workspace
@@ -1466,6 +1640,50 @@ TT_API int tt_adam_step(tt_handle_t h, void* stream, float* p, const float* g, f
     return TT_OK;
 }
 
+namespace {
+// The tensors of a list call: at least `count` arrays, no negative size, no null or unaligned pointer of a tensor that has elements.
+bool list_ok(int count, const void* array, const long long* sizes)
+{
+    const void* const* ptr = static_cast<const void* const*>(array);
+    if (count < 0 || count > (1 << 20) || (count > 0 && (!ptr || !sizes))) return false;
+    for (int i = 0; i < count; i++)
+        if (sizes[i] < 0 || (sizes[i] > 0 && (!ptr[i] || reinterpret_cast<uintptr_t>(ptr[i]) % sizeof(float) != 0))) return false;
+    return true;
+}
+}  // namespace
+
+TT_API int tt_clip_grad_norm_list(tt_handle_t h, void* stream, int count, float* const* grads, const long long* sizes,
+                                  float max_norm, float eps, int scale, float* norm_out, float* coef_out)
+{
+    if (!h) return TT_ERR_INVALID_ARG;
+    if (!list_ok(count, grads, sizes)) return fail(h, TT_ERR_INVALID_ARG, "bad clip arguments");
+    TT_BIND(h);
+    h->stats.calls++;
+    if (lists::WORKSPACE_BYTES > h->workspace_bytes) return fail(h, TT_ERR_WORKSPACE, "workspace too small for the clip");
+    const cudaError_t e = lists::launch_clip(static_cast<cudaStream_t>(stream), count, grads, sizes, max_norm, eps, scale != 0,
+                                             norm_out, coef_out, h->workspace, h->status + LIST_TICKET_WORD, h->num_sms,
+                                             &h->stats.launches);
+    if (e != cudaSuccess) return cuda_fail(h, e, "clip launch");
+    return TT_OK;
+}
+
+TT_API int tt_adam_step_list(tt_handle_t h, void* stream, int count, float* const* p, const float* const* g,
+                             float* const* m, float* const* v, const long long* sizes, float* adv,
+                             const float* grad_scale, float beta1, float beta2, float lr, float eps, float coupled_wd,
+                             float decoupled_factor, int advance)
+{
+    if (!h) return TT_ERR_INVALID_ARG;
+    if (!adv || !list_ok(count, p, sizes) || !list_ok(count, g, sizes) || !list_ok(count, m, sizes) || !list_ok(count, v, sizes))
+        return fail(h, TT_ERR_INVALID_ARG, "bad Adam arguments");
+    TT_BIND(h);
+    h->stats.calls++;
+    const cudaError_t e = lists::launch_adam(static_cast<cudaStream_t>(stream), count, p, g, m, v, sizes, adv, grad_scale,
+                                             beta1, beta2, lr, eps, coupled_wd, decoupled_factor, advance != 0,
+                                             h->status + LIST_TICKET_WORD, h->num_sms, &h->stats.launches);
+    if (e != cudaSuccess) return cuda_fail(h, e, "Adam launch");
+    return TT_OK;
+}
+
 TT_API int tt_mlp_train_step(tt_handle_t h, void* stream, const tt_mlp_desc* net, float* params, float* m,
                              float* v, float* adv, float* grads_out, const float* x, const void* target,
                              float* loss_out, int batch, float lr, float beta1, float beta2, float eps,
@@ -1581,6 +1799,10 @@ TT_API int tt_check(tt_handle_t h, void* stream)
         if (word == DEV_BAD_LABEL) {
             snprintf(h->err, sizeof(h->err), "cross-entropy label outside [0, classes): that row's loss is NaN");
             return TT_ERR_BAD_LABEL;
+        }
+        if (word == DEV_BAD_ADAPTER) {
+            snprintf(h->err, sizeof(h->err), "adapter index outside [-1, adapters): that row got no adapter");
+            return TT_ERR_BAD_ADAPTER;
         }
         snprintf(h->err, sizeof(h->err), "device-side bounded wait gave up (code %u)", word);
         return TT_ERR_DEVICE_WAIT;

@@ -1,0 +1,58 @@
+// Host entries of the low-rank adapter kernels (lora.cu), called by tt_lora_fwd / tt_lora_bwd.
+#pragma once
+#include <cuda_runtime.h>
+
+namespace tt {
+namespace lora {
+
+constexpr int MAX_RANK = 128, MAX_ADAPTERS = 4096;
+constexpr int TM = 64;                    // rows of one row tile (all of one adapter)
+
+// The adapters of a call.
+struct Adapters {
+    const float* a;       // (count, rank, K)
+    const float* b;       // (count, N, rank)
+    const float* scale;   // (count) or null: 1
+    int count, rank;
+};
+
+// Rows grouped by adapter, in device memory: perm lists the rows adapter by adapter (ascending row index within
+// one), offset[e] .. offset[e + 1] is adapter e's range of it, entry `count` holds the rows without an adapter, and
+// tile i covers tile_rows[i] entries of perm from tile_first[i] on, all of adapter tile_adapter[i] (-1: none).
+// All pointers null: every row has adapter 0, in its own order.
+struct Groups {
+    int* perm = nullptr;
+    int* offset = nullptr;        // count + 2 entries
+    int* tile_adapter = nullptr;
+    int* tile_first = nullptr;
+    int* tile_rows = nullptr;
+    int* n_tiles = nullptr;
+    int max_tiles = 0;            // launch bound: at least *n_tiles
+};
+
+// Bytes of device memory the grouping of `rows` rows over `adapters` adapters takes, and its layout inside `mem`.
+size_t groups_bytes(int rows, int adapters);
+Groups groups_layout(void* mem, int rows, int adapters);
+
+// Groups the rows.  `ticket` is a device word that is zero between launches.  An index outside [-1, adapters) counts
+// as -1 and records DEV_BAD_ADAPTER in *status.
+cudaError_t launch_group(cudaStream_t st, const Groups& g, const int* row_adapter, int rows, int adapters,
+                         unsigned int* ticket, unsigned int* status);
+
+// out[m, r] = (scaled ? scale[e_m] : 1) * sum_l x[m, l] * W_e[r, l], zeros for rows without an adapter.  W = ad.a
+// (down = true, L = K) or the transposed view of ad.b (down = false, L = N).
+cudaError_t launch_shrink(cudaStream_t st, const Groups& g, const Adapters& ad, bool down, bool scaled, const float* x,
+                          float* out, int rows, int L, int num_sms);
+
+// c[m, j] = act(c[m, j] + (scaled ? scale[e_m] : 1) * sum_r t[m, r] * W_e[j, r]), W = ad.b (up = true, J = N) or the
+// transposed view of ad.a (up = false, J = K).
+cudaError_t launch_expand(cudaStream_t st, const Groups& g, const Adapters& ad, bool up, bool scaled, const float* t,
+                          float* c, int rows, int J, int act);
+
+// da[e] = sum over e's rows of dt[m]^T x[m]   (rank, K)      skipped when da is null
+// db[e] = scale[e] * sum over e's rows of g[m]^T t[m]  (N, rank)      skipped when db is null
+cudaError_t launch_outer(cudaStream_t st, const Groups& g, const Adapters& ad, const float* dt, const float* x, float* da,
+                         const float* grad, const float* t, float* db, int rows, int N, int K, int num_sms);
+
+}  // namespace lora
+}  // namespace tt

@@ -17,6 +17,7 @@ enum : unsigned int {
     DEV_WAIT_PEER = 5,    // a wait for another GPU's flag (gradient / parameter exchange) gave up
     DEV_WAIT_STREAMK = 6, // a stream-K CTA gave up waiting for a neighbour's partial tile
     DEV_BAD_LABEL = 7,    // cross-entropy met a label outside [0, classes)
+    DEV_BAD_ADAPTER = 8,  // a row's adapter index was outside [-1, adapters)
 };
 
 // Upper bound on one wait, in nanoseconds of %globaltimer.  The longest legitimate

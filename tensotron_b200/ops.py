@@ -12,7 +12,7 @@ import math
 
 import torch
 
-from .runtime import ACT, Conv2dDesc, TensorRuntime, TensotronGemmError, broadcast_batch
+from .runtime import ACT, Conv2dDesc, LoraAdapters, TensorList, TensorRuntime, TensotronGemmError, broadcast_batch
 
 _runtime = {}
 
@@ -311,3 +311,101 @@ class Linear:
         db = torch.empty((N,), dtype=torch.float32, device=x.device) if self.Bias is not None else None
         runtime(x.device.index).LaunchLinearBackward(x, self.Weight, y, dy, dx, dw, db, M, N, K, self.act)
         return dx, dw, db
+
+
+class LoraLinear(Linear):
+    """A Linear whose rows bring their own low-rank adapters (no counterpart in the reference): `adapters` pairs
+    A (rank, in), B (out, rank) beside the one projection, y = act(x . W^T + b + Scale[e] * (x . A[e]^T) . B[e]^T) for a
+    row with adapter e.  A starts like a Linear's weight, B at zero, Scale at alpha / rank."""
+
+    def __init__(self, in_features, out_features, rank, adapters=1, alpha=None, bias=True, act=None, device="cuda", generator=None):
+        super().__init__(in_features, out_features, bias=bias, act=act, device=device, generator=generator)
+        bound = 1.0 / math.sqrt(in_features)
+        self.A = (torch.rand((adapters, rank, in_features), generator=generator) * 2 - 1).mul_(bound).to(device)
+        self.B = torch.zeros((adapters, out_features, rank), device=device)
+        self.Scale = torch.full((adapters,), (rank if alpha is None else alpha) / rank, device=device)
+
+    def _adapters(self):
+        # (made again when a tensor was replaced: the description holds addresses)
+        d = getattr(self, "_desc", None)
+        if d is None or d.a is not self.A or d.b is not self.B or d.scale is not self.Scale:
+            d = self._desc = LoraAdapters(self.A, self.B, self.Scale)
+        return d
+
+    def _check_rows(self, x, row_adapter):
+        _check(x)
+        n, k = self.Weight.shape
+        if x.dim() != 2 or x.shape[1] != k:
+            raise TensotronGemmError(1, "LoraLinear expects (rows, %d), got %s." % (k, list(x.shape)))
+        if self.A.shape[2] != k or self.B.shape[1] != n:
+            raise TensotronGemmError(1, "adapters of another layer: A %s, B %s, W %s." % (list(self.A.shape), list(self.B.shape), [n, k]))
+        if row_adapter is not None and (row_adapter.dtype != torch.int32 or not row_adapter.is_contiguous() or
+                                        row_adapter.device != x.device or tuple(row_adapter.shape) != (x.shape[0],)):
+            raise TensotronGemmError(1, "row_adapter must be %d int32 values on the rows' device." % x.shape[0])
+        return x.shape[0], n, k
+
+    def Forward(self, x, row_adapter=None):
+        """Returns (y, t): the output and the down-projected rows that Backward takes.  row_adapter: int32 (rows), -1 for a
+        row without an adapter; None: adapter 0 for every row."""
+        M, N, K = self._check_rows(x, row_adapter)
+        y = torch.empty((M, N), dtype=torch.float32, device=x.device)
+        t = torch.empty((M, self.A.shape[1]), dtype=torch.float32, device=x.device)
+        runtime(x.device.index).LaunchLoraForward(self._adapters(), row_adapter, x, self.Weight, self.Bias, y, t, M, N, K, self.act)
+        return y, t
+
+    def Backward(self, x, y, t, dy, row_adapter=None, need_dx=True, need_base=False):
+        """Returns (dx, dA, dB, dW, dbias); dW and dbias only with need_base (a frozen projection has none).  t None:
+        recomputed from x."""
+        M, N, K = self._check_rows(x, row_adapter)
+        for v, shape in ((y, (M, N)), (dy, (M, N)), (t, (M, self.A.shape[1]))):
+            if v is not None:
+                _check(v)
+                if tuple(v.shape) != shape:
+                    raise TensotronGemmError(1, "LoraLinear.Backward expects %s, got %s." % (list(shape), list(v.shape)))
+        new = lambda want, like: torch.empty_like(like) if want and like is not None else None   # noqa: E731
+        dx, da, db = new(need_dx, x), torch.empty_like(self.A), torch.empty_like(self.B)
+        dw, dbias = new(need_base, self.Weight), new(need_base, self.Bias)
+        runtime(x.device.index).LaunchLoraBackward(self._adapters(), row_adapter, x, self.Weight, y, dy, t, dx, dw, dbias, da, db,
+                                                   M, N, K, self.act)
+        return dx, da, db, dw, dbias
+
+
+def ClipGradNorm(grads, max_norm, eps=1e-6):
+    """GradUtils.ClipGradNorm (src/Tensotron/Optimizers.cs:383-422) over a list of gradients: scales all of them in place
+    by clamp(max_norm / (norm + eps), 0, 1) and returns the norm before it (device scalar)."""
+    grads = grads if isinstance(grads, TensorList) else TensorList(grads)
+    device = torch.cuda.current_device() if grads.device is None else grads.device
+    norm = torch.empty(1, dtype=torch.float32, device=torch.device("cuda", device))
+    runtime(device).LaunchClipGradNormList(grads, max_norm, eps, norm_out=norm)
+    return norm
+
+
+class Adam:
+    """Adam / AdamW over a parameter list (src/Tensotron/Optimizers.cs:144-233), one launch per step, the step counter on
+    the device.  weight_decay is coupled (added to the gradient) unless decoupled."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, decoupled=False):
+        self.Params = TensorList(params)
+        if not self.Params.count:
+            raise ValueError("Adam needs at least one parameter")
+        self.lr, self.betas, self.eps, self.weight_decay, self.decoupled = lr, betas, eps, weight_decay, decoupled
+        self.M = TensorList([torch.zeros_like(p) for p in self.Params.tensors])
+        self.V = TensorList([torch.zeros_like(p) for p in self.Params.tensors])
+        dev = self.Params.tensors[0].device
+        self.Adv = torch.zeros(3, device=dev)
+        self._norm, self._coef = torch.zeros(1, device=dev), torch.zeros(1, device=dev)
+
+    def Step(self, grads, max_norm=None, clip_eps=1e-6):
+        """One step.  max_norm: the gradients' global norm is clipped to it on the way (the tensors in `grads` stay as
+        they are); returns that norm (device scalar), else None."""
+        grads = grads if isinstance(grads, TensorList) else TensorList(grads)
+        if grads.numels != self.Params.numels:
+            raise TensotronGemmError(1, "gradients differ from the parameters in number or sizes")
+        rt = runtime(self.Params.device)
+        if max_norm is not None:
+            rt.LaunchClipGradNormList(grads, max_norm, clip_eps, norm_out=self._norm, coef_out=self._coef, scale=False)
+        coupled = 0.0 if self.decoupled else self.weight_decay
+        factor = 1.0 - self.lr * self.weight_decay if self.decoupled else 1.0
+        rt.LaunchAdamList(self.Params, grads, self.M, self.V, self.Adv, b1=self.betas[0], b2=self.betas[1], lr=self.lr, eps=self.eps,
+                          coupledWd=coupled, decoupledFactor=factor, grad_scale=self._coef if max_norm is not None else None)
+        return self._norm if max_norm is not None else None

@@ -25,6 +25,7 @@ EXPORTS = [
     "tt_peer_alloc", "tt_peer_free", "tt_peer_export", "tt_peer_open", "tt_peer_close", "tt_peer_group_create",
     "tt_peer_group_destroy", "tt_peer_linear_bwd", "tt_peer_push", "tt_peer_adam_step", "tt_peer_sync",
     "tt_peer_set_wait_limit",
+    "tt_lora_workspace", "tt_lora_fwd", "tt_lora_bwd", "tt_clip_grad_norm_list", "tt_adam_step_list",
 ]
 
 
@@ -48,6 +49,15 @@ class MlpDesc(ctypes.Structure):
 class Conv2dDesc(ctypes.Structure):
     """tt_conv2d_desc."""
     _fields_ = [(n, ctypes.c_int) for n in ("n", "c", "h", "w", "o", "kh", "kw", "stride", "padding", "dilation")]
+
+
+LORA_MAX_RANK, LORA_MAX_ADAPTERS = 128, 4096
+
+
+class LoraDesc(ctypes.Structure):
+    """tt_lora_desc."""
+    _fields_ = [("a", ctypes.c_void_p), ("b", ctypes.c_void_p), ("scale", ctypes.c_void_p),
+                ("adapters", ctypes.c_int), ("rank", ctypes.c_int)]
 
 
 class Stats(ctypes.Structure):
@@ -96,6 +106,13 @@ def load_library(path=None):
     L.tt_mse_loss.argtypes = [vp, vp, vp, vp, vp, vp, ll]
     L.tt_clip_grad_norm.argtypes = [vp, vp, vp, ll, f, f, vp]
     L.tt_mlp_train_step.argtypes = [vp, vp, ctypes.POINTER(MlpDesc), vp, vp, vp, vp, vp, vp, vp, vp, i, f, f, f, f, f, f]
+    ld, llp = ctypes.POINTER(LoraDesc), ctypes.POINTER(ll)
+    L.tt_lora_workspace.argtypes = [i] * 7
+    L.tt_lora_workspace.restype = ctypes.c_size_t
+    L.tt_lora_fwd.argtypes = [vp, vp, ld] + [vp] * 6 + [i, i, i, i]
+    L.tt_lora_bwd.argtypes = [vp, vp, ld] + [vp] * 11 + [i, i, i, i]
+    L.tt_clip_grad_norm_list.argtypes = [vp, vp, i, vp, llp, f, f, i, vp, vp]
+    L.tt_adam_step_list.argtypes = [vp, vp, i, vp, vp, vp, vp, llp, vp, vp] + [f] * 6 + [i]
     L.tt_add_into.argtypes = [vp, vp, vp, vp, ll]
     L.tt_broadcast_batch.argtypes = [i, ip, ip, i, ip, ip, ip, ip, ip, ip]
     L.tt_get_stats.argtypes = [vp, ctypes.POINTER(Stats)]
@@ -124,6 +141,44 @@ def _ptr(x):
 def _iarr(v):
     v = [int(t) for t in v]
     return (ctypes.c_int * max(1, len(v)))(*v)
+
+
+class LoraAdapters:
+    """The adapters of a Linear layer as tt_lora_fwd / tt_lora_bwd take them: a (adapters, rank, K), b (adapters, N,
+    rank), scale (adapters) or None.  Keeps the tensors alive; made once, used by every call."""
+
+    def __init__(self, a, b, scale=None):
+        for t, name in ((a, "a"), (b, "b"), (scale, "scale")):
+            if t is not None and (str(t.dtype) != "torch.float32" or not t.is_cuda or not t.is_contiguous()):
+                raise TypeError("adapter tensor %s must be a contiguous float32 CUDA tensor" % name)
+        if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
+            raise ValueError("adapters are a (adapters, rank, K) and b (adapters, N, rank), got %s and %s" % (list(a.shape), list(b.shape)))
+        if scale is not None and tuple(scale.shape) != (a.shape[0],):
+            raise ValueError("scale has one value per adapter, got %s" % list(scale.shape))
+        if any(t is not None and t.device != a.device for t in (b, scale)):
+            raise ValueError("the adapters' tensors are on different devices")
+        self.a, self.b, self.scale = a, b, scale
+        self.count, self.rank, self.device = a.shape[0], a.shape[1], a.device.index
+        self.desc = LoraDesc(a.data_ptr(), b.data_ptr(), scale.data_ptr() if scale is not None else None, self.count, self.rank)
+        self._ref = ctypes.byref(self.desc)
+
+
+class TensorList:
+    """A list of float32 CUDA tensors as the list entries take it (host arrays of addresses and sizes).  Keeps the
+    tensors alive; a program whose parameters and gradients stay where they are makes it once."""
+
+    def __init__(self, tensors):
+        self.tensors = list(tensors)
+        for t in self.tensors:
+            if str(t.dtype) != "torch.float32" or not t.is_cuda or not t.is_contiguous():
+                raise TypeError("list tensors must be contiguous float32 CUDA tensors")
+        if len({t.device for t in self.tensors}) > 1:
+            raise ValueError("the tensors of a list are on different devices")
+        self.device = self.tensors[0].device.index if self.tensors else None
+        self.count = len(self.tensors)
+        self.ptrs = (ctypes.c_void_p * max(1, self.count))(*[t.data_ptr() for t in self.tensors])
+        self.sizes = (ctypes.c_longlong * max(1, self.count))(*[t.numel() for t in self.tensors])
+        self.numels = [t.numel() for t in self.tensors]
 
 
 STATIC_CE_MAX_ROWS = 65536
@@ -312,6 +367,54 @@ class TensorRuntime:
     def LaunchClipGradNorm(self, grads, n, max_norm, eps=1e-6, norm_out=None, stream=None):
         """GradUtils.ClipGradNorm over a flat gradient span (src/Tensotron/Optimizers.cs:383-422)."""
         self._ck(self._L.tt_clip_grad_norm(self._h, self._st(stream), _ptr(grads), n, max_norm, eps, _ptr(norm_out)))
+
+    def _list(self, tensors):
+        t = tensors if isinstance(tensors, TensorList) else TensorList(tensors)
+        if t.device is not None and t.device != self.device:
+            raise TensotronGemmError(1, "the list's tensors are on device %s, this runtime is on %d" % (t.device, self.device))
+        return t
+
+    def LaunchClipGradNormList(self, grads, max_norm, eps=1e-6, norm_out=None, coef_out=None, scale=True, stream=None):
+        """GradUtils.ClipGradNorm over a list of gradients (src/Tensotron/Optimizers.cs:383-422): a TensorList or any
+        sequence of tensors.  scale=False leaves them as they are; coef_out then goes to LaunchAdamList."""
+        t = self._list(grads)
+        self._ck(self._L.tt_clip_grad_norm_list(self._h, self._st(stream), t.count, t.ptrs, t.sizes, max_norm, eps,
+                                                1 if scale else 0, _ptr(norm_out), _ptr(coef_out)))
+
+    def LaunchAdamList(self, p, g, m, v, adv, b1=0.9, b2=0.999, lr=1e-3, eps=1e-8, coupledWd=0.0, decoupledFactor=1.0,
+                       advance=True, grad_scale=None, stream=None):
+        """Adam.Step over a parameter list (src/Tensotron/Optimizers.cs:144-193) in one launch; p, g, m, v are
+        TensorLists or sequences of tensors of the same sizes."""
+        p, g, m, v = (self._list(t) for t in (p, g, m, v))
+        if not p.numels == g.numels == m.numels == v.numels:
+            raise TensotronGemmError(1, "parameters, gradients and moments differ in number or sizes")
+        self._ck(self._L.tt_adam_step_list(self._h, self._st(stream), p.count, p.ptrs, g.ptrs, m.ptrs, v.ptrs, p.sizes,
+                                           _ptr(adv), _ptr(grad_scale), b1, b2, lr, eps, coupledWd, decoupledFactor,
+                                           1 if advance else 0))
+
+    def _rows(self, adapters, row_adapter):
+        if adapters.device != self.device:
+            raise TensotronGemmError(1, "the adapters are on device %s, this runtime is on %d" % (adapters.device, self.device))
+        if row_adapter is not None and not isinstance(row_adapter, int) and str(row_adapter.dtype) != "torch.int32":
+            raise TensotronGemmError(1, "row_adapter must be int32")
+        return _ptr(row_adapter)
+
+    def LaunchLoraForward(self, adapters, row_adapter, x, w, bias, y, t, M, N, K, act=0, stream=None):
+        """tt_lora_fwd: y = act(x w^T + bias + low-rank part of each row's own adapter).  adapters: LoraAdapters;
+        row_adapter: int32 (M) or None; w None: the low-rank part is added to y; t: (M, rank) output or None."""
+        self._ck(self._L.tt_lora_fwd(self._h, self._st(stream), adapters._ref, self._rows(adapters, row_adapter), _ptr(x),
+                                     _ptr(w), _ptr(bias), _ptr(y), _ptr(t), M, N, K, ACT[act]))
+
+    def LaunchLoraBackward(self, adapters, row_adapter, x, w, y, dy, t, dx, dw, dbias, da, db, M, N, K, act=0, stream=None):
+        """tt_lora_bwd: every output may be None; w None: the low-rank part is added to dx."""
+        self._ck(self._L.tt_lora_bwd(self._h, self._st(stream), adapters._ref, self._rows(adapters, row_adapter), _ptr(x),
+                                     _ptr(w), _ptr(y), _ptr(dy), _ptr(t), _ptr(dx), _ptr(dw), _ptr(dbias), _ptr(da),
+                                     _ptr(db), M, N, K, ACT[act]))
+
+    @staticmethod
+    def LoraWorkspace(M, N, K, adapters, rank, act=0, backward=False):
+        """Bytes of the handle workspace the adapters' part of a call takes (the projection's GEMMs work behind them)."""
+        return load_library().tt_lora_workspace(M, N, K, adapters, rank, ACT[act], 1 if backward else 0)
 
     def LaunchMlpTrainStep(self, dims, act, loss_kind, params, m, v, adv, grads_out, x, target, loss, batch,
                            lr=1e-3, b1=0.9, b2=0.999, eps=1e-8, max_grad_norm=0.0, clip_eps=1e-6, stream=None):
