@@ -824,6 +824,7 @@ cudaError_t init_kernels()
                                                cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
     if (!g_generic_cluster16) cudaGetLastError();
     if (mlp_step::init_device() != 0) return cudaErrorUnknown;
+    if ((e = lora::init_rows()) != cudaSuccess) return e;
     if ((e = cudaFuncSetAttribute(skinny::skinny_n_stream_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                   skinny::stream::Cfg<4>::SMEM_BYTES)) != cudaSuccess) return e;
     if ((e = cudaFuncSetAttribute(skinny::skinny_n_stream_kernel<8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -1297,10 +1298,20 @@ TT_API int tt_lora_fwd(tt_handle_t h, void* stream, const tt_lora_desc* lora, co
     const LoraWorkspace ws = lora_workspace(M, N, lora->adapters, lora->rank, act, false);
     if (ws.end > h->workspace_bytes) return fail(h, TT_ERR_WORKSPACE, "workspace too small for the adapters");
     const lora::Adapters ad{lora->a, lora->b, lora->scale, lora->adapters, lora->rank};
+    float* tt = t ? t : reinterpret_cast<float*>(h->workspace + ws.t);
+    cudaError_t e;
+    if (h->variant == 0 && (h->math_mode == TT_MATH_FP32 || M <= 16)) {     // (strict FP32: what products with a dimension up to 16 get in every mode)
+        bool taken = false;
+        e = lora::launch_rows(st, ad, row_adapter, x, w, bias, y, tt, M, N, K, act, h->status, h->num_sms, &taken);
+        if (e != cudaSuccess) return cuda_fail(h, e, "adapter row launch");
+        if (taken) {
+            h->stats.launches += 2;
+            return TT_OK;
+        }
+    }
     lora::Groups g;
     if ((rc = lora_group(h, st, lora, row_adapter, M, ws, g))) return rc;
-    float* tt = t ? t : reinterpret_cast<float*>(h->workspace + ws.t);
-    cudaError_t e = lora::launch_shrink(st, g, ad, true, false, x, tt, M, K, h->num_sms);
+    e = lora::launch_shrink(st, g, ad, true, false, x, tt, M, K, h->num_sms);
     if (e != cudaSuccess) return cuda_fail(h, e, "adapter down-projection launch");
     h->stats.launches++;
     if (w) {

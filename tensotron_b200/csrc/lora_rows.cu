@@ -1,0 +1,347 @@
+// Forward pass of a few rows (single tokens, decode batches) through a projection with low-rank adapters:
+//     t[m] = A[e_m] x[m],    y[m] = act(w x[m] + bias + s[e_m] B[e_m] t[m])
+// in two launches.  The projection is a stream of w (4 N K bytes, read once for 16 rows), the adapters a few megabytes
+// beside it, so w's stream has to start at once and nothing may wait in front of it:
+//     rows_down_kernel   t, one CTA per row and four ranks.  It lets the next launch begin right away.
+//     rows_kernel        begins to stream w while t is still being formed, and waits for it only in front of its epilogue.
+// A warp owns NR rows of w over the whole (or the CTA's share of the) contraction, its lanes four adjacent k each; x sits in
+// shared memory, where one 128-bit load feeds 4 NR multiply-adds.  NR x MT sums per lane are added over the lanes by a
+// transposing tree (NR x MT shuffles in all).  Where x does not fit, or where cutting N alone leaves SMs idle, the CTAs of
+// a cluster cut k, and their sums are added through distributed shared memory in rank order.
+#include "lora.h"
+
+#include <cooperative_groups.h>
+#include <stdint.h>
+
+#include "ptx.cuh"
+
+namespace tt {
+namespace lora {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int THREADS = 256, WARPS = THREADS / 32;
+constexpr int MAX_X_BYTES = 160 * 1024;      // of shared memory for a CTA's share of x
+
+__device__ __forceinline__ float act_apply(float v, int act)
+{
+    if (act == 1) return v > 0.f ? v : 0.f;
+    if (act == 2) return tanhf(v);
+    return v;
+}
+
+struct RowsParams {
+    const float* x;           // (M, K)
+    const float* w;           // (N, K), or null: y holds the projection
+    const float* bias;        // (N) or null
+    const float* a;           // (count, rank, K)
+    const float* b;           // (count, N, rank)
+    const float* scale;       // (count) or null
+    const int* row_adapter;   // (M) or null
+    float* y;                 // (M, N)
+    float* t;                 // (M, rank)
+    unsigned int* status;
+    int M, N, K, rank, count, act;
+    int passes, kspan;        // row groups per warp; k per CTA of a cluster (a multiple of 128)
+};
+
+__device__ __forceinline__ int adapter_of(const RowsParams& p, int m)
+{
+    return p.row_adapter ? __ldg(p.row_adapter + m) : 0;
+}
+
+template <bool VEC>
+__device__ __forceinline__ float4 ld4(const float* p, int n)
+{
+    if (n <= 0) return make_float4(0.f, 0.f, 0.f, 0.f);
+    if (VEC) return __ldg(reinterpret_cast<const float4*>(p));
+    return make_float4(__ldg(p), n > 1 ? __ldg(p + 1) : 0.f, n > 2 ? __ldg(p + 2) : 0.f, n > 3 ? __ldg(p + 3) : 0.f);
+}
+
+constexpr int DOWN_RANKS = 4;
+
+template <bool VEC>
+__global__ void __launch_bounds__(THREADS) rows_down_kernel(const RowsParams p)
+{
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    __shared__ float red[WARPS][DOWN_RANKS];
+    const int m = blockIdx.y, r0 = blockIdx.x * DOWN_RANKS, tid = threadIdx.x;
+    const int e = adapter_of(p, m);
+    const bool has = e >= 0 && e < p.count;
+    if (!has && e != -1 && tid == 0 && p.status) atomicCAS(p.status, 0u, static_cast<unsigned int>(DEV_BAD_ADAPTER));
+    float acc[DOWN_RANKS] = {};
+    if (has) {
+        const float* x = p.x + static_cast<long long>(m) * p.K;
+        const float* a = p.a + (static_cast<long long>(e) * p.rank + r0) * p.K;
+#pragma unroll 4
+        for (int k = tid * 4; k < p.K; k += THREADS * 4) {
+            const float4 xv = ld4<VEC>(x + k, p.K - k);
+#pragma unroll
+            for (int j = 0; j < DOWN_RANKS; j++) {
+                const float4 av = ld4<VEC>(a + static_cast<long long>(j) * p.K + k, r0 + j < p.rank ? p.K - k : 0);
+                acc[j] = fmaf(xv.x, av.x, acc[j]);
+                acc[j] = fmaf(xv.y, av.y, acc[j]);
+                acc[j] = fmaf(xv.z, av.z, acc[j]);
+                acc[j] = fmaf(xv.w, av.w, acc[j]);
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < DOWN_RANKS; j++) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], o);
+        if ((tid & 31) == 0) red[tid >> 5][j] = acc[j];
+    }
+    __syncthreads();
+    if (tid < DOWN_RANKS && r0 + tid < p.rank) {
+        float s = red[0][tid];
+#pragma unroll
+        for (int w = 1; w < WARPS; w++) s += red[w][tid];
+        p.t[static_cast<long long>(m) * p.rank + r0 + tid] = s;
+    }
+}
+
+template <int NR, int MT, bool VEC>
+__global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p)
+{
+    extern __shared__ __align__(16) float rows_smem[];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int C = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int m0 = blockIdx.y * MT, mn = min(MT, p.M - m0);
+    float* xs = rows_smem;                             // [MT][kspan]
+    float* red = xs + (p.w ? MT * p.kspan : 0);        // [WARPS * NR][MT]
+    float* ts = red + WARPS * NR * MT;                 // [MT][rank], times the row's scale
+    const int k0 = rank * p.kspan, k1 = min(p.K, k0 + p.kspan);
+    const long long row0 = static_cast<long long>(blockIdx.x / C) * p.passes * WARPS * NR;
+    const int steps = p.w && k1 > k0 ? (k1 - k0 + 127) / 128 : 0;
+
+    float4 wv[NR], wn[NR];
+    const auto load_w = [&](long long n0, int step, float4 (&v)[NR]) {
+        const int k = k0 + step * 128 + lane * 4;
+#pragma unroll
+        for (int i = 0; i < NR; i++) {
+            const long long n = n0 + i;
+            v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (n < p.N && k < k1) {
+                const float* src = p.w + n * p.K + k;
+                if (VEC) v[i] = __ldcs(reinterpret_cast<const float4*>(src));
+                else     v[i] = ld4<false>(src, k1 - k);
+            }
+        }
+    };
+    if (steps > 0) load_w(row0 + warp * NR, 0, wv);
+    if (p.w) {
+        const int q4 = p.kspan / 4;
+        for (int i = tid; i < MT * q4; i += THREADS) {
+            const int m = i / q4, k = k0 + (i - m * q4) * 4;
+            const float4 v = m < mn ? ld4<VEC>(p.x + static_cast<long long>(m0 + m) * p.K + k, k1 - k) : make_float4(0.f, 0.f, 0.f, 0.f);
+            *reinterpret_cast<float4*>(xs + i * 4) = v;
+        }
+        __syncthreads();
+    }
+    bool waited = false;
+    for (int pass = 0; pass < p.passes; pass++) {
+        const long long n0 = row0 + pass * WARPS * NR, nw = n0 + warp * NR;
+        float acc[NR][MT];
+#pragma unroll
+        for (int i = 0; i < NR; i++)
+#pragma unroll
+            for (int m = 0; m < MT; m++) acc[i][m] = 0.f;
+        for (int s = 0; s < steps; s++) {
+            if (s + 1 < steps) load_w(nw, s + 1, wn);
+            else if (pass + 1 < p.passes) load_w(nw + WARPS * NR, 0, wn);
+            const float* xp = xs + s * 128 + lane * 4;
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+                const float4 xv = *reinterpret_cast<const float4*>(xp + m * p.kspan);
+#pragma unroll
+                for (int i = 0; i < NR; i++) {
+                    acc[i][m] = fmaf(wv[i].x, xv.x, acc[i][m]);
+                    acc[i][m] = fmaf(wv[i].y, xv.y, acc[i][m]);
+                    acc[i][m] = fmaf(wv[i].z, xv.z, acc[i][m]);
+                    acc[i][m] = fmaf(wv[i].w, xv.w, acc[i][m]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NR; i++) wv[i] = wn[i];
+        }
+        // transposing tree: with each step a lane keeps half of the m it holds
+        int o = 16, mine = 0;
+#pragma unroll
+        for (int h = MT / 2; h > 0; h >>= 1, o >>= 1) {
+            const bool up = (lane & o) != 0;
+            if (up) mine += h;
+#pragma unroll
+            for (int i = 0; i < NR; i++)
+#pragma unroll
+                for (int m = 0; m < h; m++) {
+                    const float send = up ? acc[i][m] : acc[i][m + h];
+                    const float keep = up ? acc[i][m + h] : acc[i][m];
+                    acc[i][m] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+                }
+        }
+        for (; o > 0; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < NR; i++) acc[i][0] += __shfl_xor_sync(0xffffffffu, acc[i][0], o);
+        if ((lane & (32 / MT - 1)) == 0) {
+#pragma unroll
+            for (int i = 0; i < NR; i++) red[(warp * NR + i) * MT + mine] = acc[i][0];
+        }
+        if (!waited) {
+            waited = true;
+            asm volatile("griddepcontrol.wait;" ::: "memory");        // t is complete from here on
+            for (int i = tid; i < mn * p.rank; i += THREADS) {
+                const int m = i / p.rank, e = adapter_of(p, m0 + m);
+                const bool has = e >= 0 && e < p.count;
+                ts[i] = has ? (p.scale ? __ldg(p.scale + e) : 1.f) * __ldcg(p.t + static_cast<long long>(m0) * p.rank + i) : 0.f;
+            }
+        }
+        if (C > 1) cluster.sync(); else __syncthreads();
+        for (int q = rank * THREADS + tid; q < WARPS * NR * mn; q += C * THREADS) {
+            const int m = q / (WARPS * NR), row = q - m * (WARPS * NR);
+            const long long n = n0 + row;
+            if (n >= p.N) continue;
+            float* out = p.y + static_cast<long long>(m0 + m) * p.N + n;
+            float v;
+            if (p.w) {
+                v = *cluster.map_shared_rank(red + row * MT + m, 0);
+                for (int c = 1; c < C; c++) v += *cluster.map_shared_rank(red + row * MT + m, c);
+                if (p.bias) v += __ldg(p.bias + n);
+            } else {
+                v = *out;
+            }
+            const int e = adapter_of(p, m0 + m);
+            if (e >= 0 && e < p.count) {
+                const float* b = p.b + (static_cast<long long>(e) * p.N + n) * p.rank;
+                const float* tr = ts + m * p.rank;
+                float u = 0.f;
+                if (VEC && (p.rank & 3) == 0) {
+#pragma unroll 4
+                    for (int r = 0; r < p.rank; r += 4) {
+                        const float4 bv = __ldg(reinterpret_cast<const float4*>(b + r));
+                        u = fmaf(tr[r], bv.x, u);
+                        u = fmaf(tr[r + 1], bv.y, u);
+                        u = fmaf(tr[r + 2], bv.z, u);
+                        u = fmaf(tr[r + 3], bv.w, u);
+                    }
+                } else {
+                    for (int r = 0; r < p.rank; r++) u = fmaf(tr[r], __ldg(b + r), u);
+                }
+                v += u;
+            }
+            *out = act_apply(v, p.act);
+        }
+        if (C > 1) cluster.sync(); else if (pass + 1 < p.passes) __syncthreads();
+    }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+template <int NR, int MT, bool VEC>
+cudaError_t launch_rows_t(cudaStream_t st, const RowsParams& p, dim3 grid, int cluster, int smem, bool init)
+{
+    if (init)
+        return cudaFuncSetAttribute(rows_kernel<NR, MT, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_ROWS_SMEM);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(THREADS, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned int>(cluster);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, rows_kernel<NR, MT, VEC>, p);
+}
+
+template <int MT, bool VEC>
+cudaError_t launch_rows_m(int nr, cudaStream_t st, const RowsParams& p, dim3 grid, int cluster, int smem, bool init)
+{
+    if constexpr (VEC) {
+        switch (nr) {
+        case 1: return launch_rows_t<1, MT, VEC>(st, p, grid, cluster, smem, init);
+        case 2: return launch_rows_t<2, MT, VEC>(st, p, grid, cluster, smem, init);
+        case 3: return launch_rows_t<3, MT, VEC>(st, p, grid, cluster, smem, init);
+        case 5: return launch_rows_t<5, MT, VEC>(st, p, grid, cluster, smem, init);
+        case 6: return launch_rows_t<6, MT, VEC>(st, p, grid, cluster, smem, init);
+        case 7: return launch_rows_t<7, MT, VEC>(st, p, grid, cluster, smem, init);
+        case 8: return launch_rows_t<8, MT, VEC>(st, p, grid, cluster, smem, init);
+        }
+    }
+    return launch_rows_t<4, MT, VEC>(st, p, grid, cluster, smem, init);
+}
+
+template <bool VEC>
+cudaError_t launch_rows_v(int mt, int nr, cudaStream_t st, const RowsParams& p, dim3 grid, int cluster, int smem, bool init)
+{
+    switch (mt) {
+    case 1: return launch_rows_m<1, VEC>(nr, st, p, grid, cluster, smem, init);
+    case 2: return launch_rows_m<2, VEC>(nr, st, p, grid, cluster, smem, init);
+    case 4: return launch_rows_m<4, VEC>(nr, st, p, grid, cluster, smem, init);
+    case 8: return launch_rows_m<8, VEC>(nr, st, p, grid, cluster, smem, init);
+    }
+    return launch_rows_m<16, VEC>(nr, st, p, grid, cluster, smem, init);
+}
+
+}  // namespace
+
+cudaError_t init_rows()
+{
+    const RowsParams none = {};
+    for (int mt = 1; mt <= 16; mt *= 2) {
+        for (int nr = 1; nr <= 8; nr++) {
+            const cudaError_t e = launch_rows_v<true>(mt, nr, nullptr, none, dim3(1), 1, 0, true);
+            if (e != cudaSuccess) return e;
+        }
+        const cudaError_t e = launch_rows_v<false>(mt, 4, nullptr, none, dim3(1), 1, 0, true);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+}
+
+cudaError_t launch_rows(cudaStream_t st, const Adapters& ad, const int* row_adapter, const float* x, const float* w,
+                        const float* bias, float* y, float* t, int M, int N, int K, int act, unsigned int* status, int num_sms,
+                        bool* taken)
+{
+    *taken = false;
+    if (M > MAX_FEW_ROWS) return cudaSuccess;
+    const int mt = M > 8 ? 16 : M > 4 ? 8 : M > 2 ? 4 : M;
+    const bool vec = K % 4 == 0 && aligned16(x) && aligned16(ad.a) && (ad.rank % 4 != 0 || aligned16(ad.b)) && (!w || aligned16(w));
+    // Cluster size, rows of w per warp and passes that give the busiest SM the least of w to read; the smallest cluster
+    // wins a tie.
+    int C = 0, nr = 1, passes = 1, kspan = 128;
+    long long best = 0;
+    for (int c = 1; c <= (w ? 8 : 1); c *= 2) {
+        const int span = ((K + c - 1) / c + 127) / 128 * 128;
+        if (w && static_cast<long long>(span) * mt * 4 > MAX_X_BYTES) continue;
+        if (c > 1 && span * (c - 1) >= K) break;                      // an empty share
+        const long long warps = static_cast<long long>(num_sms / c) * WARPS;
+        const int per = static_cast<int>((N + warps - 1) / warps);    // rows of w per warp
+        const int ps = vec ? (per + 7) / 8 : (per + 3) / 4;
+        const int r = vec ? (per + ps - 1) / ps : 4;
+        const long long cost = static_cast<long long>(ps) * r * span;
+        if (C == 0 || cost < best) { C = c; nr = r; passes = ps; kspan = span; best = cost; }
+    }
+    if (C == 0) return cudaSuccess;
+    RowsParams p{x, w, bias, ad.a, ad.b, ad.scale, row_adapter, y, t, status, M, N, K, ad.rank, ad.count, act, passes, kspan};
+    const dim3 down((ad.rank + DOWN_RANKS - 1) / DOWN_RANKS, M, 1);
+    if (vec) rows_down_kernel<true><<<down, THREADS, 0, st>>>(p);
+    else     rows_down_kernel<false><<<down, THREADS, 0, st>>>(p);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    const int smem = static_cast<int>(sizeof(float)) * ((w ? mt * kspan : 0) + WARPS * nr * mt + mt * ad.rank);
+    const int per_cluster = passes * WARPS * nr;
+    const dim3 grid(static_cast<unsigned int>((N + per_cluster - 1) / per_cluster) * C, (M + mt - 1) / mt, 1);
+    *taken = true;
+    return vec ? launch_rows_v<true>(mt, nr, st, p, grid, C, smem, false) : launch_rows_v<false>(mt, nr, st, p, grid, C, smem, false);
+}
+
+}  // namespace lora
+}  // namespace tt
