@@ -57,7 +57,7 @@ cudaError_t launch_outer(cudaStream_t st, const Groups& g, const Adapters& ad, c
 // The forward pass of at most MAX_FEW_ROWS rows in two launches (lora_rows.cu), without a grouping; *taken = false, and
 // nothing enqueued, when the call is outside what they hold.  t: (M, rank), always written.
 constexpr int MAX_FEW_ROWS = 64;
-constexpr int MAX_ROWS_SMEM = 200 * 1024;
+constexpr int MAX_ROWS_SMEM = 224 * 1024;
 cudaError_t launch_rows(cudaStream_t st, const Adapters& ad, const int* row_adapter, const float* x, const float* w,
                         const float* bias, float* y, float* t, int M, int N, int K, int act, unsigned int* status, int num_sms,
                         bool* taken);

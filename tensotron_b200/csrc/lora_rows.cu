@@ -22,7 +22,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int THREADS = 256, WARPS = THREADS / 32;
-constexpr int MAX_X_BYTES = 160 * 1024;      // of shared memory for a CTA's share of x
+constexpr int MAX_X_BYTES = 128 * 1024;      // of shared memory for a CTA's share of x
 
 __device__ __forceinline__ float act_apply(float v, int act)
 {
@@ -44,6 +44,7 @@ struct RowsParams {
     unsigned int* status;
     int M, N, K, rank, count, act;
     int passes, kspan;        // row groups per warp; k per CTA of a cluster (a multiple of 128)
+    int stages;               // steps of 128 k of the ring of w, 2 .. MAX_STAGES
 };
 
 __device__ __forceinline__ int adapter_of(const RowsParams& p, int m)
@@ -58,6 +59,34 @@ __device__ __forceinline__ float4 ld4(const float* p, int n)
     if (VEC) return __ldg(reinterpret_cast<const float4*>(p));
     return make_float4(__ldg(p), n > 1 ? __ldg(p + 1) : 0.f, n > 2 ? __ldg(p + 2) : 0.f, n > 3 ? __ldg(p + 3) : 0.f);
 }
+
+// Asynchronous copy of four floats, of which the first `n` exist (the others become 0).
+template <bool VEC>
+__device__ __forceinline__ void copy4(float* dst, const float* src, int n)
+{
+    const uint32_t d = smem_u32(dst);
+    if (VEC) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(n > 0 ? 16 : 0) : "memory");
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d + 4 * i), "l"(i < n ? src + i : src), "r"(i < n ? 4 : 0) : "memory");
+    }
+}
+
+// Waits until at most `n` of the calling thread's copy groups are unfinished.
+__device__ __forceinline__ void wait_copies(int n)
+{
+    switch (n) {
+    case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
+    case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
+    case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
+    case 3: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
+    default: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
+    }
+}
+
+constexpr int MAX_STAGES = 6;        // of the ring of w (wait_copies knows up to MAX_STAGES - 2)
 
 constexpr int DOWN_RANKS = 4;
 
@@ -113,59 +142,70 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p)
     float* xs = rows_smem;                             // [MT][kspan]
     float* red = xs + (p.w ? MT * p.kspan : 0);        // [WARPS * NR][MT]
     float* ts = red + WARPS * NR * MT;                 // [MT][rank], times the row's scale
+    float* ring = ts + ((MT * p.rank + 3) & ~3);       // [stages][WARPS][NR][128]
     const int k0 = rank * p.kspan, k1 = min(p.K, k0 + p.kspan);
     const long long row0 = static_cast<long long>(blockIdx.x / C) * p.passes * WARPS * NR;
     const int steps = p.w && k1 > k0 ? (k1 - k0 + 127) / 128 : 0;
+    const int total = steps * p.passes;
 
-    float4 wv[NR], wn[NR];
-    const auto load_w = [&](long long n0, int step, float4 (&v)[NR]) {
-        const int k = k0 + step * 128 + lane * 4;
+    // Every lane copies the four k of each of its warp's rows that it will read itself, `stages` - 1 steps ahead: no
+    // barrier is needed for w, and the bytes in flight do not take registers.
+    int is_step = 0, is_slot = 0, issued = 0;
+    long long is_row = row0 + warp * NR;
+    const auto issue = [&]() {
+        if (issued < total) {
+            const int k = k0 + is_step * 128 + lane * 4;
+            float* dst = ring + ((is_slot * WARPS + warp) * NR) * 128 + lane * 4;
 #pragma unroll
-        for (int i = 0; i < NR; i++) {
-            const long long n = n0 + i;
-            v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (n < p.N && k < k1) {
-                const float* src = p.w + n * p.K + k;
-                if (VEC) v[i] = __ldcs(reinterpret_cast<const float4*>(src));
-                else     v[i] = ld4<false>(src, k1 - k);
+            for (int i = 0; i < NR; i++) {
+                const int left = is_row + i < p.N ? k1 - k : 0;
+                copy4<VEC>(dst + i * 128, p.w + (left > 0 ? (is_row + i) * p.K + k : 0), left);
             }
+            issued++;
+            if (++is_slot == p.stages) is_slot = 0;
+            if (++is_step == steps) { is_step = 0; is_row += WARPS * NR; }
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    if (steps > 0) load_w(row0 + warp * NR, 0, wv);
-    if (p.w) {
+    if (steps > 0) {
         const int q4 = p.kspan / 4;
         for (int i = tid; i < MT * q4; i += THREADS) {
-            const int m = i / q4, k = k0 + (i - m * q4) * 4;
-            const float4 v = m < mn ? ld4<VEC>(p.x + static_cast<long long>(m0 + m) * p.K + k, k1 - k) : make_float4(0.f, 0.f, 0.f, 0.f);
-            *reinterpret_cast<float4*>(xs + i * 4) = v;
+            const int m = i / q4, k = k0 + (i - m * q4) * 4, left = m < mn ? k1 - k : 0;
+            copy4<VEC>(xs + i * 4, p.x + (left > 0 ? static_cast<long long>(m0 + m) * p.K + k : 0), left);
         }
-        __syncthreads();
+        for (int s = 0; s + 1 < p.stages; s++) issue();       // (x arrives with the first step)
     }
+    int slot = 0;
     bool waited = false;
     for (int pass = 0; pass < p.passes; pass++) {
-        const long long n0 = row0 + pass * WARPS * NR, nw = n0 + warp * NR;
+        const long long n0 = row0 + pass * WARPS * NR;
         float acc[NR][MT];
 #pragma unroll
         for (int i = 0; i < NR; i++)
 #pragma unroll
             for (int m = 0; m < MT; m++) acc[i][m] = 0.f;
         for (int s = 0; s < steps; s++) {
-            if (s + 1 < steps) load_w(nw, s + 1, wn);
-            else if (pass + 1 < p.passes) load_w(nw + WARPS * NR, 0, wn);
+            wait_copies(p.stages - 2);
+            if (s == 0 && pass == 0) __syncthreads();         // x, copied by all threads
+            const float* wp = ring + ((slot * WARPS + warp) * NR) * 128 + lane * 4;
+            if (++slot == p.stages) slot = 0;
+            float4 wv[NR];
+#pragma unroll
+            for (int i = 0; i < NR; i++) wv[i] = *reinterpret_cast<const float4*>(wp + i * 128);
             const float* xp = xs + s * 128 + lane * 4;
 #pragma unroll
             for (int m = 0; m < MT; m++) {
                 const float4 xv = *reinterpret_cast<const float4*>(xp + m * p.kspan);
 #pragma unroll
-                for (int i = 0; i < NR; i++) {
-                    acc[i][m] = fmaf(wv[i].x, xv.x, acc[i][m]);
-                    acc[i][m] = fmaf(wv[i].y, xv.y, acc[i][m]);
-                    acc[i][m] = fmaf(wv[i].z, xv.z, acc[i][m]);
-                    acc[i][m] = fmaf(wv[i].w, xv.w, acc[i][m]);
-                }
-            }
+                for (int i = 0; i < NR; i++) acc[i][m] = fmaf(wv[i].x, xv.x, acc[i][m]);
 #pragma unroll
-            for (int i = 0; i < NR; i++) wv[i] = wn[i];
+                for (int i = 0; i < NR; i++) acc[i][m] = fmaf(wv[i].y, xv.y, acc[i][m]);
+#pragma unroll
+                for (int i = 0; i < NR; i++) acc[i][m] = fmaf(wv[i].z, xv.z, acc[i][m]);
+#pragma unroll
+                for (int i = 0; i < NR; i++) acc[i][m] = fmaf(wv[i].w, xv.w, acc[i][m]);
+            }
+            issue();
         }
         // transposing tree: with each step a lane keeps half of the m it holds
         int o = 16, mine = 0;
@@ -330,13 +370,18 @@ cudaError_t launch_rows(cudaStream_t st, const Adapters& ad, const int* row_adap
         if (C == 0 || cost < best) { C = c; nr = r; passes = ps; kspan = span; best = cost; }
     }
     if (C == 0) return cudaSuccess;
-    RowsParams p{x, w, bias, ad.a, ad.b, ad.scale, row_adapter, y, t, status, M, N, K, ad.rank, ad.count, act, passes, kspan};
+    const int fixed = static_cast<int>(sizeof(float)) * ((w ? mt * kspan : 0) + WARPS * nr * mt + ((mt * ad.rank + 3) & ~3));
+    const int stage = static_cast<int>(sizeof(float)) * WARPS * nr * 128;
+    int stages = w ? (MAX_ROWS_SMEM - fixed) / stage : 0;
+    if (stages > MAX_STAGES) stages = MAX_STAGES;
+    if (w && stages < 2) return cudaSuccess;
+    RowsParams p{x, w, bias, ad.a, ad.b, ad.scale, row_adapter, y, t, status, M, N, K, ad.rank, ad.count, act, passes, kspan, stages};
     const dim3 down((ad.rank + DOWN_RANKS - 1) / DOWN_RANKS, M, 1);
     if (vec) rows_down_kernel<true><<<down, THREADS, 0, st>>>(p);
     else     rows_down_kernel<false><<<down, THREADS, 0, st>>>(p);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    const int smem = static_cast<int>(sizeof(float)) * ((w ? mt * kspan : 0) + WARPS * nr * mt + mt * ad.rank);
+    const int smem = fixed + stages * stage;
     const int per_cluster = passes * WARPS * nr;
     const dim3 grid(static_cast<unsigned int>((N + per_cluster - 1) / per_cluster) * C, (M + mt - 1) / mt, 1);
     *taken = true;
