@@ -5,7 +5,7 @@
 //     rows_down_kernel   t, one CTA per row and four ranks.  It lets the next launch begin right away.
 //     rows_kernel        begins to stream w while t is still being formed, and waits for it only in front of its epilogue.
 // A warp owns NR rows of w over the whole (or the CTA's share of the) contraction, its lanes four adjacent k each; x sits in
-// shared memory, where one 128-bit load feeds 4 NR multiply-adds.  NR x MT sums per lane are added over the lanes by a
+// shared memory in pairs of rows, where one 128-bit load feeds 4 NR multiply-adds (2 NR packed ones).  NR x MT sums per lane are added over the lanes by a
 // transposing tree (NR x MT shuffles in all).  Where x does not fit, or where cutting N alone leaves SMs idle, the CTAs of
 // a cluster cut k, and their sums are added through distributed shared memory in rank order.
 #include "lora.h"
@@ -86,6 +86,7 @@ __device__ __forceinline__ void wait_copies(int n)
     }
 }
 
+constexpr int MAX_CLUSTER = 8;
 constexpr int MAX_STAGES = 6;        // of the ring of w (wait_copies knows up to MAX_STAGES - 2)
 
 constexpr int DOWN_RANKS = 4;
@@ -134,79 +135,151 @@ __global__ void __launch_bounds__(THREADS) rows_down_kernel(const RowsParams p)
 template <int NR, int MT, bool VEC>
 __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p)
 {
+    // Up to eight rows keep two sums per output, over the even and the odd k, so that a 128-bit piece of w and one of x
+    // make two packed multiply-adds per output.  Sixteen rows would need 2 x 16 x NR registers for that: they go in pairs, x
+    // is stored pair by pair, and a packed multiply-add serves two rows.
+    constexpr bool PAIRS = MT > 8;
+    constexpr int NA = PAIRS ? MT / 2 : MT, VALUES = WARPS * NR * MT;
     extern __shared__ __align__(16) float rows_smem[];
+    __shared__ int adapter_s[MT];
+    __shared__ float scale_s[MT];
     cg::cluster_group cluster = cg::this_cluster();
     const int C = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+    if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int m0 = blockIdx.y * MT, mn = min(MT, p.M - m0);
-    float* xs = rows_smem;                             // [MT][kspan]
-    float* red = xs + (p.w ? MT * p.kspan : 0);        // [WARPS * NR][MT]
-    float* ts = red + WARPS * NR * MT;                 // [MT][rank], times the row's scale
+    float* xs = rows_smem;                             // [MT][kspan], or pairs (see below)
+    float* red = xs + (p.w ? MT * p.kspan : 0);        // [2][C][this CTA's share of the sums]
+    float* ts = red + 2 * (VALUES + MAX_CLUSTER);      // [MT][rank]
     float* ring = ts + ((MT * p.rank + 3) & ~3);       // [stages][WARPS][NR][128]
     const int k0 = rank * p.kspan, k1 = min(p.K, k0 + p.kspan);
     const long long row0 = static_cast<long long>(blockIdx.x / C) * p.passes * WARPS * NR;
     const int steps = p.w && k1 > k0 ? (k1 - k0 + 127) / 128 : 0;
     const int total = steps * p.passes;
+    const int share = (WARPS * NR * mn + C - 1) / C;   // of a pass's sums: what one CTA of the cluster finishes
 
+    int e_own = -1;
+    if (tid < mn) e_own = adapter_of(p, m0 + tid);
     // Every lane copies the four k of each of its warp's rows that it will read itself, `stages` - 1 steps ahead: no
-    // barrier is needed for w, and the bytes in flight do not take registers.
-    int is_step = 0, is_slot = 0, issued = 0;
+    // barrier is needed for w, and the bytes in flight do not take registers.  Rows behind the last one are read as
+    // the last one (their sums are not stored).
+    // The warps begin at different steps and wrap around: rows of w are often a power of two apart, and warps that walk
+    // them from the same offset in lockstep keep hitting the same memory channels.
+    const int rot = steps > 0 ? static_cast<int>((blockIdx.x / C * WARPS + warp) % static_cast<unsigned int>(steps)) : 0;
+    int is_step = rot, is_slot = 0, issued = 0, left_in_pass = steps;
     long long is_row = row0 + warp * NR;
+    const float* src[NR];
+    const auto rows_from = [&](long long n) {
+#pragma unroll
+        for (int i = 0; i < NR; i++) src[i] = p.w + min(n + i, static_cast<long long>(p.N) - 1) * p.K + k0 + lane * 4;
+    };
     const auto issue = [&]() {
         if (issued < total) {
-            const int k = k0 + is_step * 128 + lane * 4;
+            const int at = is_step * 128, left = k1 - k0 - lane * 4 - at;
             float* dst = ring + ((is_slot * WARPS + warp) * NR) * 128 + lane * 4;
 #pragma unroll
-            for (int i = 0; i < NR; i++) {
-                const int left = is_row + i < p.N ? k1 - k : 0;
-                copy4<VEC>(dst + i * 128, p.w + (left > 0 ? (is_row + i) * p.K + k : 0), left);
-            }
+            for (int i = 0; i < NR; i++) copy4<VEC>(dst + i * 128, left > 0 ? src[i] + at : p.w, left);
             issued++;
             if (++is_slot == p.stages) is_slot = 0;
-            if (++is_step == steps) { is_step = 0; is_row += WARPS * NR; }
+            if (++is_step == steps) is_step = 0;
+            if (--left_in_pass == 0) {
+                left_in_pass = steps;
+                is_row += WARPS * NR;
+                rows_from(is_row);
+            }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     if (steps > 0) {
+        rows_from(is_row);
         const int q4 = p.kspan / 4;
-        for (int i = tid; i < MT * q4; i += THREADS) {
-            const int m = i / q4, k = k0 + (i - m * q4) * 4, left = m < mn ? k1 - k : 0;
-            copy4<VEC>(xs + i * 4, p.x + (left > 0 ? static_cast<long long>(m0 + m) * p.K + k : 0), left);
+        if constexpr (PAIRS) {
+            // xs[pair][step][k 0,1 | k 2,3 of the lane][lane]: (row 0, row 1) of one k, then of the next.  Only the first step of
+            // w is asked for in front of x: x behind a full ring would arrive last.
+            issue();
+#pragma unroll 4
+            for (int i = tid; i < NA * q4; i += THREADS) {
+                const int j = i / q4, q = i - j * q4, k = k0 + q * 4;
+                const float* xr = p.x + static_cast<long long>(m0 + 2 * j) * p.K + k;
+                const float4 u = ld4<VEC>(xr, 2 * j < mn ? k1 - k : 0);
+                const float4 v = ld4<VEC>(xr + p.K, 2 * j + 1 < mn ? k1 - k : 0);
+                float* dst = xs + (j * p.kspan + (q & ~31) * 4) * 2 + (q & 31) * 4;
+                *reinterpret_cast<float4*>(dst) = make_float4(u.x, v.x, u.y, v.y);
+                *reinterpret_cast<float4*>(dst + 128) = make_float4(u.z, v.z, u.w, v.w);
+            }
+            for (int s = 1; s + 1 < p.stages; s++) issue();
+        } else {
+            for (int i = tid; i < MT * q4; i += THREADS) {
+                const int m = i / q4, k = k0 + (i - m * q4) * 4, left = m < mn ? k1 - k : 0;
+                copy4<VEC>(xs + i * 4, left > 0 ? p.x + static_cast<long long>(m0 + m) * p.K + k : p.x, left);
+            }
+            for (int s = 0; s + 1 < p.stages; s++) issue();       // (x arrives with the first step)
+            wait_copies(p.stages - 2);
         }
-        for (int s = 0; s + 1 < p.stages; s++) issue();       // (x arrives with the first step)
+    }
+    if (tid < MT) adapter_s[tid] = e_own >= 0 && e_own < p.count ? e_own : -1;
+    __syncthreads();
+    if (tid < MT) scale_s[tid] = adapter_s[tid] < 0 ? 0.f : p.scale ? __ldg(p.scale + adapter_s[tid]) : 1.f;
+    // what the first epilogue will read of B comes to L2 meanwhile
+    for (int q = rank * share + tid; q < min((rank + 1) * share, WARPS * NR * mn); q += THREADS) {
+        const int m = q / (WARPS * NR), e = adapter_s[m];
+        const long long n = row0 + (q - m * (WARPS * NR));
+        if (e >= 0 && n < p.N)
+            for (int r = 0; r < p.rank; r += 32)
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(p.b + (static_cast<long long>(e) * p.N + n) * p.rank + r));
     }
     int slot = 0;
-    bool waited = false;
     for (int pass = 0; pass < p.passes; pass++) {
         const long long n0 = row0 + pass * WARPS * NR;
-        float acc[NR][MT];
+        float2 acc2[NR][NA];
 #pragma unroll
         for (int i = 0; i < NR; i++)
 #pragma unroll
-            for (int m = 0; m < MT; m++) acc[i][m] = 0.f;
-        for (int s = 0; s < steps; s++) {
+            for (int j = 0; j < NA; j++) acc2[i][j] = make_float2(0.f, 0.f);
+        for (int done = 0, s = rot; done < steps; done++, s = s + 1 == steps ? 0 : s + 1) {
+            __syncwarp();          // (lanes that ran ahead alone would ask for their pieces of w in requests of their own)
             wait_copies(p.stages - 2);
-            if (s == 0 && pass == 0) __syncthreads();         // x, copied by all threads
             const float* wp = ring + ((slot * WARPS + warp) * NR) * 128 + lane * 4;
             if (++slot == p.stages) slot = 0;
             float4 wv[NR];
 #pragma unroll
             for (int i = 0; i < NR; i++) wv[i] = *reinterpret_cast<const float4*>(wp + i * 128);
-            const float* xp = xs + s * 128 + lane * 4;
+            if constexpr (PAIRS) {
+                const float* xp = xs + s * 256 + lane * 4;
 #pragma unroll
-            for (int m = 0; m < MT; m++) {
-                const float4 xv = *reinterpret_cast<const float4*>(xp + m * p.kspan);
+                for (int j = 0; j < NA; j++) {
+                    const float4 x01 = *reinterpret_cast<const float4*>(xp + j * 2 * p.kspan);
+                    const float4 x23 = *reinterpret_cast<const float4*>(xp + j * 2 * p.kspan + 128);
 #pragma unroll
-                for (int i = 0; i < NR; i++) acc[i][m] = fmaf(wv[i].x, xv.x, acc[i][m]);
+                    for (int i = 0; i < NR; i++) acc2[i][j] = __ffma2_rn(make_float2(wv[i].x, wv[i].x), make_float2(x01.x, x01.y), acc2[i][j]);
 #pragma unroll
-                for (int i = 0; i < NR; i++) acc[i][m] = fmaf(wv[i].y, xv.y, acc[i][m]);
+                    for (int i = 0; i < NR; i++) acc2[i][j] = __ffma2_rn(make_float2(wv[i].y, wv[i].y), make_float2(x01.z, x01.w), acc2[i][j]);
 #pragma unroll
-                for (int i = 0; i < NR; i++) acc[i][m] = fmaf(wv[i].z, xv.z, acc[i][m]);
+                    for (int i = 0; i < NR; i++) acc2[i][j] = __ffma2_rn(make_float2(wv[i].z, wv[i].z), make_float2(x23.x, x23.y), acc2[i][j]);
 #pragma unroll
-                for (int i = 0; i < NR; i++) acc[i][m] = fmaf(wv[i].w, xv.w, acc[i][m]);
+                    for (int i = 0; i < NR; i++) acc2[i][j] = __ffma2_rn(make_float2(wv[i].w, wv[i].w), make_float2(x23.z, x23.w), acc2[i][j]);
+                }
+            } else {
+                const float* xp = xs + s * 128 + lane * 4;
+#pragma unroll
+                for (int j = 0; j < NA; j++) {
+                    const float4 xv = *reinterpret_cast<const float4*>(xp + j * p.kspan);
+#pragma unroll
+                    for (int i = 0; i < NR; i++) acc2[i][j] = __ffma2_rn(make_float2(wv[i].x, wv[i].y), make_float2(xv.x, xv.y), acc2[i][j]);
+#pragma unroll
+                    for (int i = 0; i < NR; i++) acc2[i][j] = __ffma2_rn(make_float2(wv[i].z, wv[i].w), make_float2(xv.z, xv.w), acc2[i][j]);
+                }
             }
             issue();
         }
+        float acc[NR][MT];
+#pragma unroll
+        for (int i = 0; i < NR; i++)
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+                if constexpr (PAIRS) acc[i][m] = m & 1 ? acc2[i][m / 2].y : acc2[i][m / 2].x;
+                else                 acc[i][m] = acc2[i][m].x + acc2[i][m].y;
+            }
         // transposing tree: with each step a lane keeps half of the m it holds
         int o = 16, mine = 0;
 #pragma unroll
@@ -225,38 +298,35 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p)
         for (; o > 0; o >>= 1)
 #pragma unroll
             for (int i = 0; i < NR; i++) acc[i][0] += __shfl_xor_sync(0xffffffffu, acc[i][0], o);
-        if ((lane & (32 / MT - 1)) == 0) {
+        // Each sum goes to the CTA that finishes it (two buffers in turn: one barrier per pass is enough, and nobody reads
+        // another CTA's memory after it).
+        if (C > 1 && pass == 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");    // all CTAs have started
+        float* mine_red = red + (pass & 1) * (VALUES + MAX_CLUSTER);
+        if ((lane & (32 / MT - 1)) == 0 && mine < mn) {
 #pragma unroll
-            for (int i = 0; i < NR; i++) red[(warp * NR + i) * MT + mine] = acc[i][0];
-        }
-        if (!waited) {
-            waited = true;
-            asm volatile("griddepcontrol.wait;" ::: "memory");        // t is complete from here on
-            for (int i = tid; i < mn * p.rank; i += THREADS) {
-                const int m = i / p.rank, e = adapter_of(p, m0 + m);
-                const bool has = e >= 0 && e < p.count;
-                ts[i] = has ? (p.scale ? __ldg(p.scale + e) : 1.f) * __ldcg(p.t + static_cast<long long>(m0) * p.rank + i) : 0.f;
+            for (int i = 0; i < NR; i++) {
+                const int q = mine * (WARPS * NR) + warp * NR + i, owner = q / share;
+                float* dst = mine_red + rank * share + (q - owner * share);
+                *(C > 1 ? cluster.map_shared_rank(dst, owner) : dst) = acc[i][0];
             }
         }
+        if (pass == 0) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");        // t is complete from here on
+            for (int i = tid; i < mn * p.rank; i += THREADS) ts[i] = __ldcg(p.t + static_cast<long long>(m0) * p.rank + i);
+        }
         if (C > 1) cluster.sync(); else __syncthreads();
-        for (int q = rank * THREADS + tid; q < WARPS * NR * mn; q += C * THREADS) {
+        for (int q = rank * share + tid; q < min((rank + 1) * share, WARPS * NR * mn); q += THREADS) {
             const int m = q / (WARPS * NR), row = q - m * (WARPS * NR);
             const long long n = n0 + row;
             if (n >= p.N) continue;
             float* out = p.y + static_cast<long long>(m0 + m) * p.N + n;
-            float v;
-            if (p.w) {
-                v = *cluster.map_shared_rank(red + row * MT + m, 0);
-                for (int c = 1; c < C; c++) v += *cluster.map_shared_rank(red + row * MT + m, c);
-                if (p.bias) v += __ldg(p.bias + n);
-            } else {
-                v = *out;
-            }
-            const int e = adapter_of(p, m0 + m);
-            if (e >= 0 && e < p.count) {
+            float v = 0.f, u = 0.f;
+            if (!p.w) v = *out;
+            else if (p.bias) v = __ldg(p.bias + n);
+            const int e = adapter_s[m];
+            if (e >= 0) {
                 const float* b = p.b + (static_cast<long long>(e) * p.N + n) * p.rank;
                 const float* tr = ts + m * p.rank;
-                float u = 0.f;
                 if (VEC && (p.rank & 3) == 0) {
 #pragma unroll 4
                     for (int r = 0; r < p.rank; r += 4) {
@@ -269,11 +339,15 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p)
                 } else {
                     for (int r = 0; r < p.rank; r++) u = fmaf(tr[r], __ldg(b + r), u);
                 }
-                v += u;
+                u *= scale_s[m];
             }
-            *out = act_apply(v, p.act);
+            if (p.w) {
+                float z = mine_red[q - rank * share];
+                for (int c = 1; c < C; c++) z += mine_red[c * share + q - rank * share];
+                v = z + v;
+            }
+            *out = act_apply(v + u, p.act);
         }
-        if (C > 1) cluster.sync(); else if (pass + 1 < p.passes) __syncthreads();
     }
 }
 
@@ -322,8 +396,6 @@ template <bool VEC>
 cudaError_t launch_rows_v(int mt, int nr, cudaStream_t st, const RowsParams& p, dim3 grid, int cluster, int smem, bool init)
 {
     switch (mt) {
-    case 1: return launch_rows_m<1, VEC>(nr, st, p, grid, cluster, smem, init);
-    case 2: return launch_rows_m<2, VEC>(nr, st, p, grid, cluster, smem, init);
     case 4: return launch_rows_m<4, VEC>(nr, st, p, grid, cluster, smem, init);
     case 8: return launch_rows_m<8, VEC>(nr, st, p, grid, cluster, smem, init);
     }
@@ -335,7 +407,7 @@ cudaError_t launch_rows_v(int mt, int nr, cudaStream_t st, const RowsParams& p, 
 cudaError_t init_rows()
 {
     const RowsParams none = {};
-    for (int mt = 1; mt <= 16; mt *= 2) {
+    for (int mt = 4; mt <= 16; mt *= 2) {
         for (int nr = 1; nr <= 8; nr++) {
             const cudaError_t e = launch_rows_v<true>(mt, nr, nullptr, none, dim3(1), 1, 0, true);
             if (e != cudaSuccess) return e;
@@ -352,13 +424,13 @@ cudaError_t launch_rows(cudaStream_t st, const Adapters& ad, const int* row_adap
 {
     *taken = false;
     if (M > MAX_FEW_ROWS) return cudaSuccess;
-    const int mt = M > 8 ? 16 : M > 4 ? 8 : M > 2 ? 4 : M;
+    const int mt = M > 8 ? 16 : M > 4 ? 8 : 4;
     const bool vec = K % 4 == 0 && aligned16(x) && aligned16(ad.a) && (ad.rank % 4 != 0 || aligned16(ad.b)) && (!w || aligned16(w));
     // Cluster size, rows of w per warp and passes that give the busiest SM the least of w to read; the smallest cluster
     // wins a tie.
     int C = 0, nr = 1, passes = 1, kspan = 128;
     long long best = 0;
-    for (int c = 1; c <= (w ? 8 : 1); c *= 2) {
+    for (int c = 1; c <= (w ? MAX_CLUSTER : 1); c *= 2) {
         const int span = ((K + c - 1) / c + 127) / 128 * 128;
         if (w && static_cast<long long>(span) * mt * 4 > MAX_X_BYTES) continue;
         if (c > 1 && span * (c - 1) >= K) break;                      // an empty share
@@ -370,7 +442,7 @@ cudaError_t launch_rows(cudaStream_t st, const Adapters& ad, const int* row_adap
         if (C == 0 || cost < best) { C = c; nr = r; passes = ps; kspan = span; best = cost; }
     }
     if (C == 0) return cudaSuccess;
-    const int fixed = static_cast<int>(sizeof(float)) * ((w ? mt * kspan : 0) + WARPS * nr * mt + ((mt * ad.rank + 3) & ~3));
+    const int fixed = static_cast<int>(sizeof(float)) * ((w ? mt * kspan : 0) + 2 * (WARPS * nr * mt + MAX_CLUSTER) + ((mt * ad.rank + 3) & ~3));
     const int stage = static_cast<int>(sizeof(float)) * WARPS * nr * 128;
     int stages = w ? (MAX_ROWS_SMEM - fixed) / stage : 0;
     if (stages > MAX_STAGES) stages = MAX_STAGES;
