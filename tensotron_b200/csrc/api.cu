@@ -824,7 +824,7 @@ cudaError_t init_kernels()
                                                cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
     if (!g_generic_cluster16) cudaGetLastError();
     if (mlp_step::init_device() != 0) return cudaErrorUnknown;
-    if ((e = lora::init_rows()) != cudaSuccess) return e;
+    if ((e = lora::init_tiled()) != cudaSuccess || (e = lora::init_rows()) != cudaSuccess) return e;
     if ((e = cudaFuncSetAttribute(skinny::skinny_n_stream_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                   skinny::stream::Cfg<4>::SMEM_BYTES)) != cudaSuccess) return e;
     if ((e = cudaFuncSetAttribute(skinny::skinny_n_stream_kernel<8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -1319,7 +1319,7 @@ TT_API int tt_lora_fwd(tt_handle_t h, void* stream, const tt_lora_desc* lora, co
         gc.ws_off = ws.end;
         if ((rc = run_gemm(h, st, gc))) return rc;
     }
-    e = lora::launch_expand(st, g, ad, true, true, tt, y, M, N, act);
+    e = lora::launch_expand(st, g, ad, true, true, tt, y, M, N, act, h->num_sms);
     if (e != cudaSuccess) return cuda_fail(h, e, "adapter up-projection launch");
     h->stats.launches++;
     return TT_OK;
@@ -1397,7 +1397,7 @@ TT_API int tt_lora_bwd(tt_handle_t h, void* stream, const tt_lora_desc* lora, co
             gx.ws_off = ws_used;
             if ((rc = run_gemm(h, st, gx))) return rc;
         }
-        if ((e = lora::launch_expand(st, g, ad, false, false, dt, dx, M, K, TT_ACT_NONE)) != cudaSuccess)
+        if ((e = lora::launch_expand(st, g, ad, false, false, dt, dx, M, K, TT_ACT_NONE, h->num_sms)) != cudaSuccess)
             return cuda_fail(h, e, "adapter input gradient launch");
         h->stats.launches++;
     }

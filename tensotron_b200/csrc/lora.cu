@@ -14,7 +14,7 @@
 #include <cooperative_groups.h>
 #include <stdint.h>
 
-#include "ptx.cuh"
+#include "lora_common.cuh"
 
 namespace tt {
 namespace lora {
@@ -26,25 +26,6 @@ namespace {
 constexpr int THREADS = 256;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-__device__ __forceinline__ float act_apply(float v, int act)
-{
-    if (act == 1) return v > 0.f ? v : 0.f;
-    if (act == 2) return tanhf(v);
-    return v;
-}
-
-// Four consecutive floats at p, of which the first `n` exist (the others read as 0).
-__device__ __forceinline__ float4 load4(const float* p, int n, bool vec)
-{
-    if (vec && n >= 4) return __ldg(reinterpret_cast<const float4*>(p));
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (n > 0) v.x = __ldg(p);
-    if (n > 1) v.y = __ldg(p + 1);
-    if (n > 2) v.z = __ldg(p + 2);
-    if (n > 3) v.w = __ldg(p + 3);
-    return v;
-}
 
 // ---- grouping of the rows -----------------------------------------------------------------------
 
@@ -165,9 +146,11 @@ __device__ __forceinline__ Tile tile_of(const Groups& g, int i, int rows)
 // ---- shrink ---------------------------------------------------------------------------------------
 
 // A tile of 64 rows x RP ranks.  A thread owns 4 x 4 outputs; the 4 RP threads that cover the tile once form a k group,
-// and the 256 / (4 RP) k groups of the CTA share out the contraction index of every chunk of 32.  The CTAs of a cluster
-// cut the contraction into contiguous ranges; k groups are added through shared memory, the cluster's partial tiles
-// through distributed shared memory, both in ascending order.
+// and the 256 / (4 RP) k groups of the CTA share out the contraction index of every chunk of 64.  Chunks of x and of the
+// adapter arrive through a ring of asynchronous copies, both with the contraction index contiguous, so that a 128-bit
+// load of each makes two packed multiply-adds per output (sums over even and odd indices, added at the end).  The CTAs of
+// a cluster cut the contraction into contiguous ranges; k groups are added through shared memory, the cluster's partial
+// tiles through distributed shared memory, both in ascending order.
 struct ShrinkParams {
     Groups g;
     const float* x;       // (rows, L)
@@ -175,22 +158,24 @@ struct ShrinkParams {
     const float* scale;   // (count) or null
     float* out;           // (rows, rank)
     int rows, L, rank;
-    int x_vec, w_vec;     // 128-bit loads are possible
+    int x_vec, w_vec;     // 128-bit copies are possible
+};
+
+template <int RP>
+struct ShrinkCfg {
+    static constexpr int KC = 64, LD = KC + 4, STAGES = 3;
+    static constexpr int X_FLOATS = TM * LD, STAGE_FLOATS = X_FLOATS + RP * LD;
+    static constexpr int SMEM_BYTES = STAGES * STAGE_FLOATS * 4;      // (the partial tiles reuse it: 4 * 256 * 16 bytes at most)
 };
 
 template <int RP, bool KMAJ>
 __global__ void __launch_bounds__(THREADS) shrink_kernel(const ShrinkParams p)
 {
-    constexpr int KC = 32, LD = KC + 4, GROUP = 4 * RP, KG = THREADS / GROUP, QPG = KC / 4 / KG;
-    constexpr int X_FLOATS = TM * LD, W_FLOATS = KMAJ ? RP * LD : KC * (RP + 4);
-    constexpr int RED_FLOATS = KG * TM * RP;
-    constexpr int SMEM = X_FLOATS + W_FLOATS > RED_FLOATS ? X_FLOATS + W_FLOATS : RED_FLOATS;
-    constexpr int XL = TM * KC / 4 / THREADS;                       // float4 of x per thread and chunk
-    constexpr int WL = (RP * KC / 4 + THREADS - 1) / THREADS;
-    __shared__ __align__(16) float smem[SMEM];
+    using C = ShrinkCfg<RP>;
+    constexpr int KC = C::KC, LD = C::LD, GROUP = 4 * RP, KG = THREADS / GROUP, QPG = KC / 4 / KG;
+    constexpr int XL = TM * KC / 4 / THREADS;                       // copies of x per thread and chunk
+    extern __shared__ __align__(16) float smem[];
     __shared__ int row_s[TM];
-    float* xs = smem;
-    float* ws = smem + X_FLOATS;
     cg::cluster_group cluster = cg::this_cluster();
     const int S = static_cast<int>(cluster.num_blocks()), split = static_cast<int>(cluster.block_rank());
     const int tid = threadIdx.x;
@@ -201,86 +186,82 @@ __global__ void __launch_bounds__(THREADS) shrink_kernel(const ShrinkParams p)
     __syncthreads();
     const int span = ((p.L + S - 1) / S + KC - 1) / KC * KC;
     const int l0 = split * span, l1 = tile.adapter < 0 ? 0 : min(p.L, l0 + span);
+    const int chunks = l1 > l0 ? (l1 - l0 + KC - 1) / KC : 0;
     const float* w = p.w + (tile.adapter < 0 ? 0ll : static_cast<long long>(tile.adapter) * p.rank * p.L);
 
-    float4 xr[XL], wr[WL];
-    const auto fetch = [&](int l) {
+    const int xc = (tid % (KC / 4)) * 4;
+    const float* xsrc[XL];
 #pragma unroll
-        for (int i = 0; i < XL; i++) {
-            const int q = tid + i * THREADS, r = q / (KC / 4), c = l + (q % (KC / 4)) * 4;
-            xr[i] = row_s[r] < 0 ? make_float4(0.f, 0.f, 0.f, 0.f)
-                                 : load4(p.x + static_cast<long long>(row_s[r]) * p.L + c, l1 - c, p.x_vec);
-        }
+    for (int i = 0; i < XL; i++) {
+        const int r = row_s[tid / (KC / 4) + i * (THREADS / (KC / 4))];
+        xsrc[i] = r < 0 ? nullptr : p.x + static_cast<long long>(r) * p.L + l0 + xc;
+    }
+    const auto issue = [&](int chunk) {
+        if (chunk < chunks) {
+            float* xs = smem + (chunk % C::STAGES) * C::STAGE_FLOATS;
+            float* ws = xs + C::X_FLOATS;
+            const int l = l0 + chunk * KC;
 #pragma unroll
-        for (int i = 0; i < WL; i++) {
-            const int q = tid + i * THREADS;
-            wr[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (q < RP * KC / 4) {
-                if (KMAJ) {
-                    const int r = q / (KC / 4), c = l + (q % (KC / 4)) * 4;
-                    if (rb + r < p.rank) wr[i] = load4(w + static_cast<long long>(rb + r) * p.L + c, l1 - c, p.w_vec);
-                } else {
-                    const int c = l + q / (RP / 4), r = rb + (q % (RP / 4)) * 4;
-                    if (c < l1) wr[i] = load4(w + static_cast<long long>(c) * p.rank + r, p.rank - r, p.w_vec);
+            for (int i = 0; i < XL; i++) {
+                const int left = xsrc[i] ? l1 - l - xc : 0;
+                copy4(xs + (tid / (KC / 4) + i * (THREADS / (KC / 4))) * LD + xc, left > 0 ? xsrc[i] + chunk * KC : p.x, left, p.x_vec);
+            }
+            if (KMAJ) {
+#pragma unroll
+                for (int q = tid; q < RP * KC / 4; q += THREADS) {
+                    const int r = q / (KC / 4), c = (q % (KC / 4)) * 4, left = rb + r < p.rank ? l1 - l - c : 0;
+                    copy4(ws + r * LD + c, left > 0 ? w + static_cast<long long>(rb + r) * p.L + l + c : p.w, left, p.w_vec);
+                }
+            } else {
+#pragma unroll 4
+                for (int q = tid; q < RP * KC; q += THREADS) {
+                    const int c = q / RP, r = q % RP;
+                    const bool there = l + c < l1 && rb + r < p.rank;
+                    copy1(ws + r * LD + c, there ? w + static_cast<long long>(l + c) * p.rank + rb + r : p.w, there);
                 }
             }
         }
+        commit_copies();
     };
 
     const int kg = tid / GROUP, t = tid % GROUP, rg = t % 16, cgp = t / 16;
-    float acc[4][4];
+    float2 acc[4][4];
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) acc[i][j] = 0.f;
-    if (l0 < l1) fetch(l0);
-    for (int l = l0; l < l1; l += KC) {
-#pragma unroll
-        for (int i = 0; i < XL; i++) {
-            const int q = tid + i * THREADS;
-            *reinterpret_cast<float4*>(xs + (q / (KC / 4)) * LD + (q % (KC / 4)) * 4) = xr[i];
-        }
-#pragma unroll
-        for (int i = 0; i < WL; i++) {
-            const int q = tid + i * THREADS;
-            if (q < RP * KC / 4) {
-                if (KMAJ) *reinterpret_cast<float4*>(ws + (q / (KC / 4)) * LD + (q % (KC / 4)) * 4) = wr[i];
-                else      *reinterpret_cast<float4*>(ws + (q / (RP / 4)) * (RP + 4) + (q % (RP / 4)) * 4) = wr[i];
-            }
-        }
+        for (int j = 0; j < 4; j++) acc[i][j] = make_float2(0.f, 0.f);
+    for (int s = 0; s < C::STAGES - 1; s++) issue(s);
+    for (int chunk = 0; chunk < chunks; chunk++) {
+        wait_copies<C::STAGES - 2>();
         __syncthreads();
-        if (l + KC < l1) fetch(l + KC);
+        issue(chunk + C::STAGES - 1);
+        const float* xs = smem + (chunk % C::STAGES) * C::STAGE_FLOATS;
+        const float* ws = xs + C::X_FLOATS;
 #pragma unroll
         for (int qq = 0; qq < QPG; qq++) {
             const int k = (kg * QPG + qq) * 4;
-            float xv[4][4], wv[4][4];                    // [row][k], [rank][k]
+            float4 xv[4], wv[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) xv[i] = *reinterpret_cast<const float4*>(xs + (rg + 16 * i) * LD + k);
+#pragma unroll
+            for (int j = 0; j < 4; j++) wv[j] = *reinterpret_cast<const float4*>(ws + (cgp + RP / 4 * j) * LD + k);
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                *reinterpret_cast<float4*>(xv[i]) = *reinterpret_cast<const float4*>(xs + (rg + 16 * i) * LD + k);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if (KMAJ) {
-                    *reinterpret_cast<float4*>(wv[j]) = *reinterpret_cast<const float4*>(ws + (cgp + RP / 4 * j) * LD + k);
-                } else {
-                    const float4 v = *reinterpret_cast<const float4*>(ws + (k + j) * (RP + 4) + cgp * 4);
-                    wv[0][j] = v.x; wv[1][j] = v.y; wv[2][j] = v.z; wv[3][j] = v.w;
-                }
-            }
+                for (int j = 0; j < 4; j++) acc[i][j] = __ffma2_rn(make_float2(xv[i].x, xv[i].y), make_float2(wv[j].x, wv[j].y), acc[i][j]);
 #pragma unroll
-            for (int kk = 0; kk < 4; kk++)
+            for (int i = 0; i < 4; i++)
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) acc[i][j] = fmaf(xv[i][kk], wv[j][kk], acc[i][j]);
+                for (int j = 0; j < 4; j++) acc[i][j] = __ffma2_rn(make_float2(xv[i].z, xv[i].w), make_float2(wv[j].z, wv[j].w), acc[i][j]);
         }
-        __syncthreads();
     }
+    wait_copies<0>();
+    __syncthreads();
     // partial tiles [kg][row][rank]
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            smem[(kg * TM + rg + 16 * i) * RP + (KMAJ ? cgp + RP / 4 * j : cgp * 4 + j)] = acc[i][j];
+        for (int j = 0; j < 4; j++) smem[(kg * TM + rg + 16 * i) * RP + cgp + RP / 4 * j] = acc[i][j].x + acc[i][j].y;
     __syncthreads();
     for (int e = tid; e < TM * RP && KG > 1; e += THREADS) {
         float s = smem[e];
@@ -303,86 +284,114 @@ __global__ void __launch_bounds__(THREADS) shrink_kernel(const ShrinkParams p)
 
 // ---- expand ---------------------------------------------------------------------------------------
 
-// A tile of 64 rows x 128 columns; a warp owns 8 rows, a lane 4 adjacent columns of each.  Ranks are taken 32 at a
-// time.  Bound by the read and write of c; its values are fetched before the products are formed.
+// 64 rows x `tiles_per` column tiles of 128; a warp owns 8 rows, a lane 4 adjacent columns of each.  Bound by the read and
+// write of c, so what a step needs (the tile of c, read and written by the same thread, and up to RC ranks of the adapter)
+// arrives through a two-stage ring of asynchronous copies while the step before it is computed and stored; the rows' t and
+// the row numbers are read once per CTA.  More than RC ranks take several steps per column tile.
 struct ExpandParams {
     Groups g;
     const float* t;       // (rows, rank)
     const float* w;       // RMAJ: (count, J, rank), else (count, rank, J)
     const float* scale;   // (count) or null
     float* c;             // (rows, J)
-    int rows, J, rank, act;
+    int rows, J, rank, act, tiles_per;
     int w_vec, c_vec;
 };
 
 constexpr int EN = 128;
 
+template <int RC>
+struct ExpandCfg {
+    static constexpr int STAGES = 2, LD = EN + 4, C_FLOATS = TM * EN, STAGE_FLOATS = C_FLOATS + RC * LD;
+    static int smem_bytes(int rank) { return (STAGES * STAGE_FLOATS + TM * ((rank + RC - 1) / RC * RC)) * 4; }
+};
+
 template <int RC, bool RMAJ>
-__global__ void __launch_bounds__(THREADS) expand_kernel(const ExpandParams p)
+__global__ void __launch_bounds__(THREADS, 2) expand_kernel(const ExpandParams p)
 {
-    __shared__ __align__(16) float ts[TM][RC];
-    __shared__ __align__(16) float ws[RC][EN + 4];
+    using C = ExpandCfg<RC>;
+    extern __shared__ __align__(16) float smem[];
     __shared__ int row_s[TM];
     const Tile tile = tile_of(p.g, blockIdx.x, p.rows);
     if (!tile.valid || (tile.adapter < 0 && p.act == 0)) return;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rchunks = (p.rank + RC - 1) / RC, rpad = rchunks * RC;
+    float* ts = smem + C::STAGES * C::STAGE_FLOATS;          // [TM][rpad], scaled
     if (tid < TM) row_s[tid] = tid < tile.rows ? (p.g.perm ? __ldg(p.g.perm + tile.first + tid) : tile.first + tid) : -1;
     __syncthreads();
-    const int j0 = blockIdx.y * EN, j = j0 + lane * 4, left = p.J - j;
-    float4 cv[8];
+    const int ct0 = blockIdx.y * p.tiles_per, ct1 = min((p.J + EN - 1) / EN, ct0 + p.tiles_per);
+    const int steps = (ct1 - ct0) * rchunks;
+    const float* w = p.w + static_cast<long long>(tile.adapter < 0 ? 0 : tile.adapter) * p.rank * p.J;
+    float* crow[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         const int m = row_s[warp * 8 + i];
-        cv[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (m >= 0) {
-            const float* src = p.c + static_cast<long long>(m) * p.J + j;
-            if (p.c_vec && left >= 4) {
-                cv[i] = *reinterpret_cast<const float4*>(src);
-            } else {
-                if (left > 0) cv[i].x = src[0];
-                if (left > 1) cv[i].y = src[1];
-                if (left > 2) cv[i].z = src[2];
-                if (left > 3) cv[i].w = src[3];
+        crow[i] = m < 0 ? nullptr : p.c + static_cast<long long>(m) * p.J;
+    }
+    const auto issue = [&](int step) {
+        if (step < steps) {
+            const int ct = ct0 + step / rchunks, rc = step % rchunks, j0 = ct * EN, r0 = rc * RC;
+            float* cs = smem + (step % C::STAGES) * C::STAGE_FLOATS;
+            float* ws = cs + C::C_FLOATS;
+            if (rc == 0) {                                   // (stays in its stage for this step; kept in registers for the others)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int left = crow[i] ? p.J - j0 - lane * 4 : 0;
+                    copy4(cs + (warp * 8 + i) * EN + lane * 4, left > 0 ? crow[i] + j0 + lane * 4 : p.c, left, p.c_vec);
+                }
+            }
+            if (tile.adapter >= 0) {
+                if (RMAJ) {
+                    // B is read along its ranks and stored rank by rank
+#pragma unroll 4
+                    for (int q = tid; q < EN * RC; q += THREADS) {
+                        const int n = q / RC, r = q % RC;
+                        const bool there = j0 + n < p.J && r0 + r < p.rank;
+                        copy1(ws + r * C::LD + n, there ? w + static_cast<long long>(j0 + n) * p.rank + r0 + r : p.w, there);
+                    }
+                } else {
+#pragma unroll
+                    for (int q = tid; q < RC * (EN / 4); q += THREADS) {
+                        const int r = q / (EN / 4), n = (q % (EN / 4)) * 4, left = r0 + r < p.rank ? p.J - j0 - n : 0;
+                        copy4(ws + r * C::LD + n, left > 0 ? w + static_cast<long long>(r0 + r) * p.J + j0 + n : p.w, left, p.w_vec);
+                    }
+                }
             }
         }
-    }
-    float4 acc[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        commit_copies();
+    };
+    issue(0);
     if (tile.adapter >= 0) {
-        const float* w = p.w + static_cast<long long>(tile.adapter) * p.rank * p.J;
         const float scale = p.scale ? __ldg(p.scale + tile.adapter) : 1.f;
-        for (int r0 = 0; r0 < p.rank; r0 += RC) {
-            const int rn = min(RC, p.rank - r0);
-            if (r0) __syncthreads();
-            for (int e = tid; e < TM * RC; e += THREADS) {
-                const int r = e / RC, c = e % RC;
-                ts[r][c] = row_s[r] >= 0 && c < rn ? scale * __ldg(p.t + static_cast<long long>(row_s[r]) * p.rank + r0 + c) : 0.f;
+        for (int e = tid; e < TM * rpad; e += THREADS) {
+            const int r = e / rpad, c = e - r * rpad;
+            ts[e] = row_s[r] >= 0 && c < p.rank ? scale * __ldg(p.t + static_cast<long long>(row_s[r]) * p.rank + c) : 0.f;
+        }
+    }
+    float4 cv[8], acc[8];
+    for (int step = 0; step < steps; step++) {
+        issue(step + 1);
+        wait_copies<1>();
+        __syncthreads();
+        const int rc = step % rchunks, j = (ct0 + step / rchunks) * EN + lane * 4, left = p.J - j;
+        const float* cs = smem + (step % C::STAGES) * C::STAGE_FLOATS;
+        const float* ws = cs + C::C_FLOATS;
+        if (rc == 0) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                cv[i] = *reinterpret_cast<const float4*>(cs + (warp * 8 + i) * EN + lane * 4);
+                acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
             }
-            if (RMAJ) {
-                for (int e = tid; e < EN * (RC / 4); e += THREADS) {
-                    const int n = e / (RC / 4), r = (e % (RC / 4)) * 4;
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (j0 + n < p.J) v = load4(w + static_cast<long long>(j0 + n) * p.rank + r0 + r, rn - r, p.w_vec);
-                    ws[r][n] = v.x; ws[r + 1][n] = v.y; ws[r + 2][n] = v.z; ws[r + 3][n] = v.w;
-                }
-            } else {
-                for (int e = tid; e < RC * (EN / 4); e += THREADS) {
-                    const int r = e / (EN / 4), n = (e % (EN / 4)) * 4;
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (r < rn) v = load4(w + static_cast<long long>(r0 + r) * p.J + j0 + n, p.J - j0 - n, p.w_vec);
-                    *reinterpret_cast<float4*>(&ws[r][n]) = v;
-                }
-            }
-            __syncthreads();
+        }
+        if (tile.adapter >= 0) {
 #pragma unroll
             for (int r = 0; r < RC; r += 4) {
                 float4 wv[4];
 #pragma unroll
-                for (int q = 0; q < 4; q++) wv[q] = *reinterpret_cast<const float4*>(&ws[r + q][lane * 4]);
+                for (int q = 0; q < 4; q++) wv[q] = *reinterpret_cast<const float4*>(ws + (r + q) * C::LD + lane * 4);
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const float4 tv = *reinterpret_cast<const float4*>(&ts[warp * 8 + i][r]);
+                    const float4 tv = *reinterpret_cast<const float4*>(ts + (warp * 8 + i) * rpad + rc * RC + r);
                     const float t4[4] = {tv.x, tv.y, tv.z, tv.w};
 #pragma unroll
                     for (int q = 0; q < 4; q++) {
@@ -394,25 +403,27 @@ __global__ void __launch_bounds__(THREADS) expand_kernel(const ExpandParams p)
                 }
             }
         }
-    }
+        if (rc == rchunks - 1) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int m = row_s[warp * 8 + i];
-        if (m < 0) continue;
-        float4 v = make_float4(cv[i].x + acc[i].x, cv[i].y + acc[i].y, cv[i].z + acc[i].z, cv[i].w + acc[i].w);
-        if (p.act) {
-            v.x = act_apply(v.x, p.act); v.y = act_apply(v.y, p.act);
-            v.z = act_apply(v.z, p.act); v.w = act_apply(v.w, p.act);
+            for (int i = 0; i < 8; i++) {
+                if (!crow[i]) continue;
+                float4 v = make_float4(cv[i].x + acc[i].x, cv[i].y + acc[i].y, cv[i].z + acc[i].z, cv[i].w + acc[i].w);
+                if (p.act) {
+                    v.x = act_apply(v.x, p.act); v.y = act_apply(v.y, p.act);
+                    v.z = act_apply(v.z, p.act); v.w = act_apply(v.w, p.act);
+                }
+                float* dst = crow[i] + j;
+                if (p.c_vec && left >= 4) {
+                    *reinterpret_cast<float4*>(dst) = v;
+                } else {
+                    if (left > 0) dst[0] = v.x;
+                    if (left > 1) dst[1] = v.y;
+                    if (left > 2) dst[2] = v.z;
+                    if (left > 3) dst[3] = v.w;
+                }
+            }
         }
-        float* dst = p.c + static_cast<long long>(m) * p.J + j;
-        if (p.c_vec && left >= 4) {
-            *reinterpret_cast<float4*>(dst) = v;
-        } else {
-            if (left > 0) dst[0] = v.x;
-            if (left > 1) dst[1] = v.y;
-            if (left > 2) dst[2] = v.z;
-            if (left > 3) dst[3] = v.w;
-        }
+        __syncthreads();
     }
 }
 
@@ -420,14 +431,15 @@ __global__ void __launch_bounds__(THREADS) expand_kernel(const ExpandParams p)
 
 // out = small^T . big over one adapter's rows: a tile of RP ranks x 128 columns.  A thread owns 8 ranks x 4 columns; the
 // 4 RP threads that cover the tile once form a row group, and the row groups of the CTA share out the rows of every
-// chunk of 32.  The CTAs of a cluster cut the adapter's rows into contiguous ranges.  Joins as in shrink_kernel.  Two
-// jobs in one grid: dA (rank, K) from dt and x, dB (N, rank) from t and g.
+// chunk of 32, which arrive through a ring of asynchronous copies.  The CTAs of a cluster cut the adapter's rows into
+// contiguous ranges.  Joins as in shrink_kernel.  Two jobs in one grid: dA (rank, K) from dt and x, dB (N, rank) from t
+// and g.
 struct OuterJob {
     const float* small;   // (rows, rank)
     const float* big;     // (rows, C)
     float* out;           // (count, rank, C), or (count, C, rank) when col_major
     const float* scale;   // (count) or null
-    int C, col_major, tiles, big_vec;
+    int C, col_major, tiles, big_vec, small_vec;
 };
 
 struct OuterParams {
@@ -437,15 +449,19 @@ struct OuterParams {
 };
 
 template <int RP>
+struct OuterCfg {
+    static constexpr int MC = 32, CN = 128, STAGES = 3, STAGE_FLOATS = MC * CN + MC * RP;
+    static constexpr int RED_FLOATS = THREADS / (4 * RP) * RP * CN;
+    static constexpr int SMEM_BYTES = (STAGES * STAGE_FLOATS > RED_FLOATS ? STAGES * STAGE_FLOATS : RED_FLOATS) * 4;
+};
+
+template <int RP>
 __global__ void __launch_bounds__(THREADS) outer_kernel(const OuterParams p)
 {
-    constexpr int MC = 32, CN = 128, GROUP = 4 * RP, MG = THREADS / GROUP;
-    constexpr int RED_FLOATS = MG * RP * CN, IN_FLOATS = MC * CN + MC * RP;
-    constexpr int SMEM = RED_FLOATS > IN_FLOATS ? RED_FLOATS : IN_FLOATS;
-    constexpr int BL = MC * CN / 4 / THREADS, SL = (MC * RP + THREADS - 1) / THREADS;
-    __shared__ __align__(16) float smem[SMEM];
-    float* bs = smem;
-    float* ss = smem + MC * CN;
+    using C = OuterCfg<RP>;
+    constexpr int MC = C::MC, CN = C::CN, GROUP = 4 * RP, MG = THREADS / GROUP;
+    constexpr int BL = MC * CN / 4 / THREADS;
+    extern __shared__ __align__(16) float smem[];
     cg::cluster_group cluster = cg::this_cluster();
     const int S = static_cast<int>(cluster.num_blocks()), split = static_cast<int>(cluster.block_rank());
     const int tid = threadIdx.x, e = blockIdx.y, rb = blockIdx.z * RP;
@@ -462,37 +478,42 @@ __global__ void __launch_bounds__(THREADS) outer_kernel(const OuterParams p)
     }
     const int span = ((n + S - 1) / S + MC - 1) / MC * MC;
     const int m0 = split * span, m1 = min(n, m0 + span);
+    const int chunks = m1 > m0 ? (m1 - m0 + MC - 1) / MC : 0;
 
-    float4 br[BL];
-    float sr[SL];
-    const auto row_of = [&](int m) { return p.g.perm ? __ldg(p.g.perm + first + m) : m; };
-    const auto fetch = [&](int m) {
+    const auto issue = [&](int chunk) {
+        if (chunk < chunks) {
+            float* bs = smem + (chunk % C::STAGES) * C::STAGE_FLOATS;
+            float* ss = bs + MC * CN;
+            const int m = m0 + chunk * MC;
+            const int cl = (tid % (CN / 4)) * 4;
 #pragma unroll
-        for (int i = 0; i < BL; i++) {
-            const int q = tid + i * THREADS, r = m + q / (CN / 4), c = c0 + (q % (CN / 4)) * 4;
-            br[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (r < m1) br[i] = load4(job.big + static_cast<long long>(row_of(r)) * job.C + c, job.C - c, job.big_vec);
-        }
+            for (int i = 0; i < BL; i++) {
+                const int r = tid / (CN / 4) + i * (THREADS / (CN / 4));
+                const int left = m + r < m1 ? job.C - c0 - cl : 0;
+                const long long row = left > 0 ? (p.g.perm ? __ldg(p.g.perm + first + m + r) : m + r) : 0;
+                copy4(bs + r * CN + cl, left > 0 ? job.big + row * job.C + c0 + cl : job.big, left, job.big_vec);
+            }
 #pragma unroll
-        for (int i = 0; i < SL; i++) {
-            const int q = tid + i * THREADS, r = m + q / RP, c = rb + q % RP;
-            sr[i] = 0.f;
-            if (q < MC * RP && r < m1 && c < p.rank) sr[i] = __ldg(job.small + static_cast<long long>(row_of(r)) * p.rank + c);
+            for (int q = tid; q < MC * RP / 4; q += THREADS) {
+                const int r = q / (RP / 4), c = rb + (q % (RP / 4)) * 4;
+                const int left = m + r < m1 ? p.rank - c : 0;
+                const long long row = left > 0 ? (p.g.perm ? __ldg(p.g.perm + first + m + r) : m + r) : 0;
+                copy4(ss + q * 4, left > 0 ? job.small + row * p.rank + c : job.small, left, job.small_vec);
+            }
         }
+        commit_copies();
     };
     const int mg = tid / GROUP, t = tid % GROUP, cl = t % 32, rg = t / 32;   // rg: 8 ranks, cl: 4 columns
     float4 acc[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (m0 < m1) fetch(m0);
-    for (int m = m0; m < m1; m += MC) {
-#pragma unroll
-        for (int i = 0; i < BL; i++) *reinterpret_cast<float4*>(bs + (tid + i * THREADS) * 4) = br[i];
-#pragma unroll
-        for (int i = 0; i < SL; i++)
-            if (tid + i * THREADS < MC * RP) ss[tid + i * THREADS] = sr[i];
+    for (int s = 0; s < C::STAGES - 1; s++) issue(s);
+    for (int chunk = 0; chunk < chunks; chunk++) {
+        wait_copies<C::STAGES - 2>();
         __syncthreads();
-        if (m + MC < m1) fetch(m + MC);
+        issue(chunk + C::STAGES - 1);
+        const float* bs = smem + (chunk % C::STAGES) * C::STAGE_FLOATS;
+        const float* ss = bs + MC * CN;
 #pragma unroll 4
         for (int r = mg; r < MC; r += MG) {
             const float4 bv = *reinterpret_cast<const float4*>(bs + r * CN + cl * 4);
@@ -507,8 +528,9 @@ __global__ void __launch_bounds__(THREADS) outer_kernel(const OuterParams p)
                 acc[i].w = fmaf(sv[i], bv.w, acc[i].w);
             }
         }
-        __syncthreads();
     }
+    wait_copies<0>();
+    __syncthreads();
     // partial tiles [mg][rank][column]
 #pragma unroll
     for (int i = 0; i < 8; i++) *reinterpret_cast<float4*>(smem + (mg * RP + rg * 8 + i) * CN + cl * 4) = acc[i];
@@ -538,9 +560,10 @@ __global__ void __launch_bounds__(THREADS) outer_kernel(const OuterParams p)
 }
 
 template <typename P>
-cudaError_t launch_cluster(cudaStream_t st, void (*kernel)(P), dim3 grid, int cluster, const P& p)
+cudaError_t launch_cluster(cudaStream_t st, void (*kernel)(P), dim3 grid, int cluster, int smem, const P& p)
 {
     cudaLaunchConfig_t cfg = {};
+    cfg.dynamicSmemBytes = smem;
     cfg.gridDim = grid;
     cfg.blockDim = dim3(THREADS, 1, 1);
     cfg.stream = st;
@@ -606,7 +629,7 @@ cudaError_t launch_shrink(cudaStream_t st, const Groups& g, const Adapters& ad, 
     p.out = out;
     p.rows = rows; p.L = L; p.rank = ad.rank;
     p.x_vec = aligned16(x) && L % 4 == 0;
-    p.w_vec = aligned16(p.w) && (down ? L : ad.rank) % 4 == 0;
+    p.w_vec = down && aligned16(p.w) && L % 4 == 0;
     const int tiles = g.perm ? g.max_tiles : (rows + TM - 1) / TM;
     const int rp = ad.rank <= 8 ? 8 : ad.rank <= 16 ? 16 : ad.rank <= 32 ? 32 : 64;
     const int rblocks = (ad.rank + rp - 1) / rp;
@@ -614,19 +637,19 @@ cudaError_t launch_shrink(cudaStream_t st, const Groups& g, const Adapters& ad, 
     while (S < 8 && static_cast<long long>(tiles) * rblocks * S < 3ll * num_sms && L / (2 * S) >= 64) S *= 2;
     const dim3 grid(static_cast<unsigned int>(tiles) * S, rblocks, 1);
     if (down) {
-        if (rp == 8)       return launch_cluster(st, shrink_kernel<8, true>, grid, S, p);
-        else if (rp == 16) return launch_cluster(st, shrink_kernel<16, true>, grid, S, p);
-        else if (rp == 32) return launch_cluster(st, shrink_kernel<32, true>, grid, S, p);
-        return launch_cluster(st, shrink_kernel<64, true>, grid, S, p);
+        if (rp == 8)       return launch_cluster(st, shrink_kernel<8, true>, grid, S, ShrinkCfg<8>::SMEM_BYTES, p);
+        else if (rp == 16) return launch_cluster(st, shrink_kernel<16, true>, grid, S, ShrinkCfg<16>::SMEM_BYTES, p);
+        else if (rp == 32) return launch_cluster(st, shrink_kernel<32, true>, grid, S, ShrinkCfg<32>::SMEM_BYTES, p);
+        return launch_cluster(st, shrink_kernel<64, true>, grid, S, ShrinkCfg<64>::SMEM_BYTES, p);
     }
-    if (rp == 8)       return launch_cluster(st, shrink_kernel<8, false>, grid, S, p);
-    else if (rp == 16) return launch_cluster(st, shrink_kernel<16, false>, grid, S, p);
-    else if (rp == 32) return launch_cluster(st, shrink_kernel<32, false>, grid, S, p);
-    return launch_cluster(st, shrink_kernel<64, false>, grid, S, p);
+    if (rp == 8)       return launch_cluster(st, shrink_kernel<8, false>, grid, S, ShrinkCfg<8>::SMEM_BYTES, p);
+    else if (rp == 16) return launch_cluster(st, shrink_kernel<16, false>, grid, S, ShrinkCfg<16>::SMEM_BYTES, p);
+    else if (rp == 32) return launch_cluster(st, shrink_kernel<32, false>, grid, S, ShrinkCfg<32>::SMEM_BYTES, p);
+    return launch_cluster(st, shrink_kernel<64, false>, grid, S, ShrinkCfg<64>::SMEM_BYTES, p);
 }
 
 cudaError_t launch_expand(cudaStream_t st, const Groups& g, const Adapters& ad, bool up, bool scaled, const float* t,
-                          float* c, int rows, int J, int act)
+                          float* c, int rows, int J, int act, int num_sms)
 {
     ExpandParams p;
     p.g = g;
@@ -635,20 +658,22 @@ cudaError_t launch_expand(cudaStream_t st, const Groups& g, const Adapters& ad, 
     p.scale = scaled ? ad.scale : nullptr;
     p.c = c;
     p.rows = rows; p.J = J; p.rank = ad.rank; p.act = act;
-    p.w_vec = aligned16(p.w) && (up ? ad.rank : J) % 4 == 0;
+    p.w_vec = !up && aligned16(p.w) && J % 4 == 0;
     p.c_vec = aligned16(c) && J % 4 == 0;
-    const int tiles = g.perm ? g.max_tiles : (rows + TM - 1) / TM;
-    const dim3 grid(tiles, (J + EN - 1) / EN, 1);
-    if (grid.y > 65535u) return cudaErrorInvalidValue;
+    const int tiles = g.perm ? g.max_tiles : (rows + TM - 1) / TM, cols = (J + EN - 1) / EN;
+    // column tiles per CTA: as many as leave four CTAs per SM
+    long long per = static_cast<long long>(tiles) * cols / (4ll * num_sms);
+    p.tiles_per = static_cast<int>(per < 1 ? 1 : per > 8 ? 8 : per);
+    const dim3 grid(tiles, (cols + p.tiles_per - 1) / p.tiles_per, 1);
     const int rc = ad.rank <= 8 ? 8 : ad.rank <= 16 ? 16 : 32;
     if (up) {
-        if (rc == 8)       expand_kernel<8, true><<<grid, THREADS, 0, st>>>(p);
-        else if (rc == 16) expand_kernel<16, true><<<grid, THREADS, 0, st>>>(p);
-        else               expand_kernel<32, true><<<grid, THREADS, 0, st>>>(p);
+        if (rc == 8)       expand_kernel<8, true><<<grid, THREADS, ExpandCfg<8>::smem_bytes(ad.rank), st>>>(p);
+        else if (rc == 16) expand_kernel<16, true><<<grid, THREADS, ExpandCfg<16>::smem_bytes(ad.rank), st>>>(p);
+        else               expand_kernel<32, true><<<grid, THREADS, ExpandCfg<32>::smem_bytes(ad.rank), st>>>(p);
     } else {
-        if (rc == 8)       expand_kernel<8, false><<<grid, THREADS, 0, st>>>(p);
-        else if (rc == 16) expand_kernel<16, false><<<grid, THREADS, 0, st>>>(p);
-        else               expand_kernel<32, false><<<grid, THREADS, 0, st>>>(p);
+        if (rc == 8)       expand_kernel<8, false><<<grid, THREADS, ExpandCfg<8>::smem_bytes(ad.rank), st>>>(p);
+        else if (rc == 16) expand_kernel<16, false><<<grid, THREADS, ExpandCfg<16>::smem_bytes(ad.rank), st>>>(p);
+        else               expand_kernel<32, false><<<grid, THREADS, ExpandCfg<32>::smem_bytes(ad.rank), st>>>(p);
     }
     return cudaGetLastError();
 }
@@ -662,8 +687,8 @@ cudaError_t launch_outer(cudaStream_t st, const Groups& g, const Adapters& ad, c
     p.rank = ad.rank;
     int jobs = 0;
     p.job[0].tiles = p.job[1].tiles = 0;
-    if (da) p.job[jobs++] = OuterJob{dt, x, da, nullptr, K, 0, (K + 127) / 128, aligned16(x) && K % 4 == 0};
-    if (db) p.job[jobs++] = OuterJob{t, grad, db, ad.scale, N, 1, (N + 127) / 128, aligned16(grad) && N % 4 == 0};
+    if (da) p.job[jobs++] = OuterJob{dt, x, da, nullptr, K, 0, (K + 127) / 128, aligned16(x) && K % 4 == 0, aligned16(dt) && ad.rank % 4 == 0};
+    if (db) p.job[jobs++] = OuterJob{t, grad, db, ad.scale, N, 1, (N + 127) / 128, aligned16(grad) && N % 4 == 0, aligned16(t) && ad.rank % 4 == 0};
     if (jobs == 0) return cudaSuccess;
     if (jobs == 1) { p.job[1] = p.job[0]; p.job[1].tiles = 0; }
     const int rp = ad.rank <= 8 ? 8 : ad.rank <= 16 ? 16 : ad.rank <= 32 ? 32 : 64;
@@ -674,10 +699,41 @@ cudaError_t launch_outer(cudaStream_t st, const Groups& g, const Adapters& ad, c
     while (S < 8 && static_cast<long long>(tiles) * rblocks * groups * S < 3ll * num_sms && rows / (2 * S * groups) >= 32) S *= 2;
     // (without a grouping the adapters behind the first have no rows: their CTAs store zeros)
     const dim3 grid(static_cast<unsigned int>(tiles) * S, ad.count, rblocks);
-    if (rp == 8)       return launch_cluster(st, outer_kernel<8>, grid, S, p);
-    else if (rp == 16) return launch_cluster(st, outer_kernel<16>, grid, S, p);
-    else if (rp == 32) return launch_cluster(st, outer_kernel<32>, grid, S, p);
-    return launch_cluster(st, outer_kernel<64>, grid, S, p);
+    if (rp == 8)       return launch_cluster(st, outer_kernel<8>, grid, S, OuterCfg<8>::SMEM_BYTES, p);
+    else if (rp == 16) return launch_cluster(st, outer_kernel<16>, grid, S, OuterCfg<16>::SMEM_BYTES, p);
+    else if (rp == 32) return launch_cluster(st, outer_kernel<32>, grid, S, OuterCfg<32>::SMEM_BYTES, p);
+    return launch_cluster(st, outer_kernel<64>, grid, S, OuterCfg<64>::SMEM_BYTES, p);
+}
+
+namespace {
+template <typename K>
+cudaError_t allow_smem(K* kernel, int bytes) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); }
+
+template <int RP>
+cudaError_t init_rank()
+{
+    cudaError_t e;
+    if ((e = allow_smem(shrink_kernel<RP, true>, ShrinkCfg<RP>::SMEM_BYTES)) != cudaSuccess) return e;
+    if ((e = allow_smem(shrink_kernel<RP, false>, ShrinkCfg<RP>::SMEM_BYTES)) != cudaSuccess) return e;
+    return allow_smem(outer_kernel<RP>, OuterCfg<RP>::SMEM_BYTES);
+}
+
+template <int RC>
+cudaError_t init_expand()
+{
+    const int bytes = ExpandCfg<RC>::smem_bytes(RC == 32 ? MAX_RANK : RC);
+    const cudaError_t e = allow_smem(expand_kernel<RC, true>, bytes);
+    return e != cudaSuccess ? e : allow_smem(expand_kernel<RC, false>, bytes);
+}
+}  // namespace
+
+cudaError_t init_tiled()
+{
+    cudaError_t e;
+    if ((e = init_rank<8>()) != cudaSuccess || (e = init_rank<16>()) != cudaSuccess || (e = init_rank<32>()) != cudaSuccess ||
+        (e = init_rank<64>()) != cudaSuccess || (e = init_expand<8>()) != cudaSuccess || (e = init_expand<16>()) != cudaSuccess)
+        return e;
+    return init_expand<32>();
 }
 
 }  // namespace lora

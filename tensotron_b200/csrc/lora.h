@@ -47,7 +47,7 @@ cudaError_t launch_shrink(cudaStream_t st, const Groups& g, const Adapters& ad, 
 // c[m, j] = act(c[m, j] + (scaled ? scale[e_m] : 1) * sum_r t[m, r] * W_e[j, r]), W = ad.b (up = true, J = N) or the
 // transposed view of ad.a (up = false, J = K).
 cudaError_t launch_expand(cudaStream_t st, const Groups& g, const Adapters& ad, bool up, bool scaled, const float* t,
-                          float* c, int rows, int J, int act);
+                          float* c, int rows, int J, int act, int num_sms);
 
 // da[e] = sum over e's rows of dt[m]^T x[m]   (rank, K)      skipped when da is null
 // db[e] = scale[e] * sum over e's rows of g[m]^T t[m]  (N, rank)      skipped when db is null
@@ -61,7 +61,9 @@ constexpr int MAX_ROWS_SMEM = 224 * 1024;
 cudaError_t launch_rows(cudaStream_t st, const Adapters& ad, const int* row_adapter, const float* x, const float* w,
                         const float* bias, float* y, float* t, int M, int N, int K, int act, unsigned int* status, int num_sms,
                         bool* taken);
-cudaError_t init_rows();      // kernel attributes, once per context (called from tt_create)
+// Kernel attributes, once per context (called from tt_create).
+cudaError_t init_tiled();
+cudaError_t init_rows();
 
 }  // namespace lora
 }  // namespace tt

@@ -13,7 +13,7 @@
 #include <cooperative_groups.h>
 #include <stdint.h>
 
-#include "ptx.cuh"
+#include "lora_common.cuh"
 
 namespace tt {
 namespace lora {
@@ -23,13 +23,6 @@ namespace cg = cooperative_groups;
 
 constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int MAX_X_BYTES = 128 * 1024;      // of shared memory for a CTA's share of x
-
-__device__ __forceinline__ float act_apply(float v, int act)
-{
-    if (act == 1) return v > 0.f ? v : 0.f;
-    if (act == 2) return tanhf(v);
-    return v;
-}
 
 struct RowsParams {
     const float* x;           // (M, K)
@@ -60,34 +53,20 @@ __device__ __forceinline__ float4 ld4(const float* p, int n)
     return make_float4(__ldg(p), n > 1 ? __ldg(p + 1) : 0.f, n > 2 ? __ldg(p + 2) : 0.f, n > 3 ? __ldg(p + 3) : 0.f);
 }
 
-// Asynchronous copy of four floats, of which the first `n` exist (the others become 0).
-template <bool VEC>
-__device__ __forceinline__ void copy4(float* dst, const float* src, int n)
-{
-    const uint32_t d = smem_u32(dst);
-    if (VEC) {
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(n > 0 ? 16 : 0) : "memory");
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d + 4 * i), "l"(i < n ? src + i : src), "r"(i < n ? 4 : 0) : "memory");
-    }
-}
-
 // Waits until at most `n` of the calling thread's copy groups are unfinished.
-__device__ __forceinline__ void wait_copies(int n)
+__device__ __forceinline__ void wait_copies_n(int n)
 {
     switch (n) {
-    case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
-    case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
-    case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
-    case 3: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
-    default: asm volatile("cp.async.wait_group 4;" ::: "memory"); break;
+    case 0: wait_copies<0>(); break;
+    case 1: wait_copies<1>(); break;
+    case 2: wait_copies<2>(); break;
+    case 3: wait_copies<3>(); break;
+    default: wait_copies<4>(); break;
     }
 }
 
 constexpr int MAX_CLUSTER = 8;
-constexpr int MAX_STAGES = 6;        // of the ring of w (wait_copies knows up to MAX_STAGES - 2)
+constexpr int MAX_STAGES = 6;        // of the ring of w (wait_copies_n knows up to MAX_STAGES - 2)
 
 constexpr int DOWN_RANKS = 4;
 
@@ -178,7 +157,7 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p)
             const int at = is_step * 128, left = k1 - k0 - lane * 4 - at;
             float* dst = ring + ((is_slot * WARPS + warp) * NR) * 128 + lane * 4;
 #pragma unroll
-            for (int i = 0; i < NR; i++) copy4<VEC>(dst + i * 128, left > 0 ? src[i] + at : p.w, left);
+            for (int i = 0; i < NR; i++) copy4(dst + i * 128, left > 0 ? src[i] + at : p.w, left, VEC);
             issued++;
             if (++is_slot == p.stages) is_slot = 0;
             if (++is_step == steps) is_step = 0;
@@ -188,7 +167,7 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p)
                 rows_from(is_row);
             }
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        commit_copies();
     };
     if (steps > 0) {
         rows_from(is_row);
@@ -211,10 +190,10 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p)
         } else {
             for (int i = tid; i < MT * q4; i += THREADS) {
                 const int m = i / q4, k = k0 + (i - m * q4) * 4, left = m < mn ? k1 - k : 0;
-                copy4<VEC>(xs + i * 4, left > 0 ? p.x + static_cast<long long>(m0 + m) * p.K + k : p.x, left);
+                copy4(xs + i * 4, left > 0 ? p.x + static_cast<long long>(m0 + m) * p.K + k : p.x, left, VEC);
             }
             for (int s = 0; s + 1 < p.stages; s++) issue();       // (x arrives with the first step)
-            wait_copies(p.stages - 2);
+            wait_copies_n(p.stages - 2);
         }
     }
     if (tid < MT) adapter_s[tid] = e_own >= 0 && e_own < p.count ? e_own : -1;
@@ -238,7 +217,7 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p)
             for (int j = 0; j < NA; j++) acc2[i][j] = make_float2(0.f, 0.f);
         for (int done = 0, s = rot; done < steps; done++, s = s + 1 == steps ? 0 : s + 1) {
             __syncwarp();          // (lanes that ran ahead alone would ask for their pieces of w in requests of their own)
-            wait_copies(p.stages - 2);
+            wait_copies_n(p.stages - 2);
             const float* wp = ring + ((slot * WARPS + warp) * NR) * 128 + lane * 4;
             if (++slot == p.stages) slot = 0;
             float4 wv[NR];
