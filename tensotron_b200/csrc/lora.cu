@@ -143,14 +143,28 @@ __device__ __forceinline__ Tile tile_of(const Groups& g, int i, int rows)
     return t;
 }
 
+// Rows of a tile as their numbers in the call, -1 behind the last one.
+__device__ __forceinline__ void tile_row_numbers(const Groups& g, const Tile& tile, int* row_s)
+{
+    if (threadIdx.x < TM)
+        row_s[threadIdx.x] = static_cast<int>(threadIdx.x) < tile.rows ? (g.perm ? __ldg(g.perm + tile.first + threadIdx.x) : tile.first + static_cast<int>(threadIdx.x)) : -1;
+}
+
+// The tiled kernels take their operands through rings of stages filled by asynchronous copies, of 16 bytes where every row
+// starts on such a boundary and is a multiple of 16 bytes long (VEC), else of 4.  Every thread copies the same places of
+// every stage, so that a copy costs an addition and the instruction itself.  (Bulk copies, one per row of a stage, were
+// tried: about 45 cycles each per SM whatever their length, 8192 x 4096 rows in 104 us against 55.)  Rows behind the last one
+// of a tile repeat its first (their outputs are not stored); what lies behind the last index of a contraction is 0 or is
+// not looked at.
+
 // ---- shrink ---------------------------------------------------------------------------------------
 
-// A tile of 64 rows x RP ranks.  A thread owns 4 x 4 outputs; the 4 RP threads that cover the tile once form a k group,
-// and the 256 / (4 RP) k groups of the CTA share out the contraction index of every chunk of 64.  Chunks of x and of the
-// adapter arrive through a ring of asynchronous copies, both with the contraction index contiguous, so that a 128-bit
-// load of each makes two packed multiply-adds per output (sums over even and odd indices, added at the end).  The CTAs of
-// a cluster cut the contraction into contiguous ranges; k groups are added through shared memory, the cluster's partial
-// tiles through distributed shared memory, both in ascending order.
+// A tile of 64 rows x RP ranks.  A thread owns 4 rows x 8 ranks; the 2 RP threads that cover the tile once form a k group,
+// and the 128 / RP k groups of the CTA share out the contraction index of every chunk of 64.  KMAJ: both operands
+// have the contraction index contiguous, a 128-bit load of each makes two packed multiply-adds per output (sums over even
+// and odd indices, added at the end); otherwise the ranks are contiguous and a packed multiply-add serves two of them.  The
+// CTAs of a cluster cut the contraction into contiguous ranges; k groups are added through shared memory, the cluster's
+// partial tiles through distributed shared memory, both in ascending order.
 struct ShrinkParams {
     Groups g;
     const float* x;       // (rows, L)
@@ -158,22 +172,27 @@ struct ShrinkParams {
     const float* scale;   // (count) or null
     float* out;           // (rows, rank)
     int rows, L, rank;
-    int x_vec, w_vec;     // 128-bit copies are possible
-};
-
-template <int RP>
-struct ShrinkCfg {
-    static constexpr int KC = 64, LD = KC + 4, STAGES = 3;
-    static constexpr int X_FLOATS = TM * LD, STAGE_FLOATS = X_FLOATS + RP * LD;
-    static constexpr int SMEM_BYTES = STAGES * STAGE_FLOATS * 4;      // (the partial tiles reuse it: 4 * 256 * 16 bytes at most)
 };
 
 template <int RP, bool KMAJ>
-__global__ void __launch_bounds__(THREADS) shrink_kernel(const ShrinkParams p)
+struct ShrinkCfg {
+    static constexpr int KC = 64, LD = KC + 4, STAGES = 4, X_FLOATS = TM * LD;
+    static constexpr int RED_FLOATS = 128 / RP * TM * RP;
+    // row pitch of the adapter's part of a stage, and its floats (ranks behind the last one are read past a row's end)
+    __host__ __device__ static int pitch(int rank) { return KMAJ ? LD : (rank + 3) & ~3; }
+    __host__ __device__ static int w_floats(int rank) { return KMAJ ? RP * LD : KC * pitch(rank) + RP; }
+    static int smem_bytes(int rank)
+    {
+        const int ring = STAGES * (X_FLOATS + w_floats(rank));
+        return (ring > RED_FLOATS ? ring : RED_FLOATS) * 4;
+    }
+};
+
+template <int RP, bool KMAJ, bool VEC>
+__global__ void __launch_bounds__(THREADS, 2) shrink_kernel(const ShrinkParams p)
 {
-    using C = ShrinkCfg<RP>;
-    constexpr int KC = C::KC, LD = C::LD, GROUP = 4 * RP, KG = THREADS / GROUP, QPG = KC / 4 / KG;
-    constexpr int XL = TM * KC / 4 / THREADS;                       // copies of x per thread and chunk
+    using C = ShrinkCfg<RP, KMAJ>;
+    constexpr int KC = C::KC, LD = C::LD, STAGES = C::STAGES, GROUP = 2 * RP, KG = THREADS / GROUP, QPG = KC / 4 / KG;
     extern __shared__ __align__(16) float smem[];
     __shared__ int row_s[TM];
     cg::cluster_group cluster = cg::this_cluster();
@@ -182,42 +201,65 @@ __global__ void __launch_bounds__(THREADS) shrink_kernel(const ShrinkParams p)
     const int rb = blockIdx.y * RP;                                  // first rank of this block of ranks
     const Tile tile = tile_of(p.g, blockIdx.x / S, p.rows);
     if (!tile.valid) return;                                         // (the whole cluster)
-    if (tid < TM) row_s[tid] = tid < tile.rows ? (p.g.perm ? __ldg(p.g.perm + tile.first + tid) : tile.first + tid) : -1;
+    tile_row_numbers(p.g, tile, row_s);
     __syncthreads();
     const int span = ((p.L + S - 1) / S + KC - 1) / KC * KC;
     const int l0 = split * span, l1 = tile.adapter < 0 ? 0 : min(p.L, l0 + span);
     const int chunks = l1 > l0 ? (l1 - l0 + KC - 1) / KC : 0;
+    const int pitch = C::pitch(p.rank), stage_floats = C::X_FLOATS + C::w_floats(p.rank);
     const float* w = p.w + (tile.adapter < 0 ? 0ll : static_cast<long long>(tile.adapter) * p.rank * p.L);
+    const int wrows = min(RP, p.rank - rb);
 
-    const int xc = (tid % (KC / 4)) * 4;
-    const float* xsrc[XL];
+    // VEC: this thread's places of a stage
+    constexpr int Q = KC / 4, XN = TM * Q / THREADS, WN = (RP * Q + THREADS - 1) / THREADS;
+    const int c4 = (tid % Q) * 4, xr = tid / Q;
+    const float* xsrc[XN];
+    const float* wsrc[WN];
+    if constexpr (VEC) {
 #pragma unroll
-    for (int i = 0; i < XL; i++) {
-        const int r = row_s[tid / (KC / 4) + i * (THREADS / (KC / 4))];
-        xsrc[i] = r < 0 ? nullptr : p.x + static_cast<long long>(r) * p.L + l0 + xc;
+        for (int i = 0; i < XN; i++) {
+            const int r = row_s[xr + i * (THREADS / Q)];
+            xsrc[i] = p.x + static_cast<long long>(r < 0 ? row_s[0] : r) * p.L + l0 + c4;
+        }
+#pragma unroll
+        for (int i = 0; i < WN; i++) {
+            if constexpr (KMAJ) wsrc[i] = w + static_cast<long long>(rb + min(xr + i * (THREADS / Q), wrows - 1)) * p.L + l0 + c4;
+            else                wsrc[i] = w + static_cast<long long>(l0) * p.rank + (tid + i * THREADS) * 4;
+        }
     }
     const auto issue = [&](int chunk) {
         if (chunk < chunks) {
-            float* xs = smem + (chunk % C::STAGES) * C::STAGE_FLOATS;
+            float* xs = smem + (chunk % STAGES) * stage_floats;
             float* ws = xs + C::X_FLOATS;
-            const int l = l0 + chunk * KC;
+            const int l = l0 + chunk * KC, kn = min(KC, l1 - l);
+            if constexpr (VEC) {
+                if (c4 < kn) {
 #pragma unroll
-            for (int i = 0; i < XL; i++) {
-                const int left = xsrc[i] ? l1 - l - xc : 0;
-                copy4(xs + (tid / (KC / 4) + i * (THREADS / (KC / 4))) * LD + xc, left > 0 ? xsrc[i] + chunk * KC : p.x, left, p.x_vec);
-            }
-            if (KMAJ) {
+                    for (int i = 0; i < XN; i++) copy16(xs + (xr + i * (THREADS / Q)) * LD + c4, xsrc[i] + chunk * KC);
+                    if constexpr (KMAJ) {
 #pragma unroll
-                for (int q = tid; q < RP * KC / 4; q += THREADS) {
-                    const int r = q / (KC / 4), c = (q % (KC / 4)) * 4, left = rb + r < p.rank ? l1 - l - c : 0;
-                    copy4(ws + r * LD + c, left > 0 ? w + static_cast<long long>(rb + r) * p.L + l + c : p.w, left, p.w_vec);
+                        for (int i = 0; i < WN; i++)
+                            if (RP * Q >= THREADS || xr < RP) copy16(ws + (xr + i * (THREADS / Q)) * LD + c4, wsrc[i] + chunk * KC);
+                    }
+                }
+                if constexpr (!KMAJ) {
+                    // (all ranks of kn steps: one dense block)
+                    const int n4 = kn * p.rank / 4;
+                    const long long at = static_cast<long long>(chunk) * KC * p.rank;
+                    for (int q = tid, i = 0; q < n4; q += THREADS, i++) copy16(ws + q * 4, wsrc[0] + at + i * (THREADS * 4));
                 }
             } else {
-#pragma unroll 4
+                for (int q = tid; q < TM * KC; q += THREADS) {
+                    const int r = q / KC, c = q % KC;
+                    const bool there = c < kn && row_s[r] >= 0;
+                    copy1(xs + r * LD + c, there ? p.x + static_cast<long long>(row_s[r]) * p.L + l + c : p.x, there);
+                }
                 for (int q = tid; q < RP * KC; q += THREADS) {
-                    const int c = q / RP, r = q % RP;
-                    const bool there = l + c < l1 && rb + r < p.rank;
-                    copy1(ws + r * LD + c, there ? w + static_cast<long long>(l + c) * p.rank + rb + r : p.w, there);
+                    const int r = KMAJ ? q / KC : q % RP, c = KMAJ ? q % KC : q / RP;
+                    const bool there = c < kn && r < wrows;
+                    if (KMAJ || there || rb + r < pitch)
+                        copy1(KMAJ ? ws + r * LD + c : ws + c * pitch + rb + r,
+                              there ? w + (KMAJ ? static_cast<long long>(rb + r) * p.L + l + c : static_cast<long long>(l + c) * p.rank + rb + r) : p.w, there);
                 }
             }
         }
@@ -225,34 +267,50 @@ __global__ void __launch_bounds__(THREADS) shrink_kernel(const ShrinkParams p)
     };
 
     const int kg = tid / GROUP, t = tid % GROUP, rg = t % 16, cgp = t / 16;
-    float2 acc[4][4];
+    float2 acc[4][8];                          // KMAJ: (even, odd) sums per rank; else [4][0..3]: rank pairs
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) acc[i][j] = make_float2(0.f, 0.f);
-    for (int s = 0; s < C::STAGES - 1; s++) issue(s);
-    for (int chunk = 0; chunk < chunks; chunk++) {
-        wait_copies<C::STAGES - 2>();
+        for (int j = 0; j < 8; j++) acc[i][j] = make_float2(0.f, 0.f);
+    for (int s = 0; s < STAGES - 1; s++) issue(s);
+    for (int done = 0; done < chunks; done++) {
+        wait_copies<STAGES - 2>();
         __syncthreads();
-        issue(chunk + C::STAGES - 1);
-        const float* xs = smem + (chunk % C::STAGES) * C::STAGE_FLOATS;
-        const float* ws = xs + C::X_FLOATS;
+        issue(done + STAGES - 1);
+        const float* xs = smem + (done % STAGES) * stage_floats;
+        const float* ws = xs + C::X_FLOATS + (KMAJ ? 0 : rb);
+        const int kn = min(KC, l1 - l0 - done * KC);
 #pragma unroll
         for (int qq = 0; qq < QPG; qq++) {
             const int k = (kg * QPG + qq) * 4;
-            float4 xv[4], wv[4];
+            if (k >= kn) break;
+            float4 xv[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) xv[i] = *reinterpret_cast<const float4*>(xs + (rg + 16 * i) * LD + k);
+            if constexpr (KMAJ) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) wv[j] = *reinterpret_cast<const float4*>(ws + (cgp + RP / 4 * j) * LD + k);
+                for (int j = 0; j < 8; j++) {
+                    const float4 wv = *reinterpret_cast<const float4*>(ws + (cgp + RP / 8 * j) * LD + k);
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+                    for (int i = 0; i < 4; i++) acc[i][j] = __ffma2_rn(make_float2(xv[i].x, xv[i].y), make_float2(wv.x, wv.y), acc[i][j]);
 #pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j] = __ffma2_rn(make_float2(xv[i].x, xv[i].y), make_float2(wv[j].x, wv[j].y), acc[i][j]);
+                    for (int i = 0; i < 4; i++) acc[i][j] = __ffma2_rn(make_float2(xv[i].z, xv[i].w), make_float2(wv.z, wv.w), acc[i][j]);
+                }
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+                for (int kk = 0; kk < 4; kk++) {
+                    const float4 w0 = *reinterpret_cast<const float4*>(ws + (k + kk) * pitch + cgp * 8);
+                    const float4 w1 = *reinterpret_cast<const float4*>(ws + (k + kk) * pitch + cgp * 8 + 4);
 #pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j] = __ffma2_rn(make_float2(xv[i].z, xv[i].w), make_float2(wv[j].z, wv[j].w), acc[i][j]);
+                    for (int i = 0; i < 4; i++) {
+                        const float xk = kk == 0 ? xv[i].x : kk == 1 ? xv[i].y : kk == 2 ? xv[i].z : xv[i].w;
+                        acc[i][0] = __ffma2_rn(make_float2(xk, xk), make_float2(w0.x, w0.y), acc[i][0]);
+                        acc[i][1] = __ffma2_rn(make_float2(xk, xk), make_float2(w0.z, w0.w), acc[i][1]);
+                        acc[i][2] = __ffma2_rn(make_float2(xk, xk), make_float2(w1.x, w1.y), acc[i][2]);
+                        acc[i][3] = __ffma2_rn(make_float2(xk, xk), make_float2(w1.z, w1.w), acc[i][3]);
+                    }
+                }
+            }
         }
     }
     wait_copies<0>();
@@ -261,7 +319,9 @@ __global__ void __launch_bounds__(THREADS) shrink_kernel(const ShrinkParams p)
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) smem[(kg * TM + rg + 16 * i) * RP + cgp + RP / 4 * j] = acc[i][j].x + acc[i][j].y;
+        for (int j = 0; j < 8; j++)
+            smem[(kg * TM + rg + 16 * i) * RP + (KMAJ ? cgp + RP / 8 * j : cgp * 8 + j)] =
+                KMAJ ? acc[i][j].x + acc[i][j].y : (j & 1 ? acc[i][j / 2].y : acc[i][j / 2].x);
     __syncthreads();
     for (int e = tid; e < TM * RP && KG > 1; e += THREADS) {
         float s = smem[e];
@@ -285,9 +345,10 @@ __global__ void __launch_bounds__(THREADS) shrink_kernel(const ShrinkParams p)
 // ---- expand ---------------------------------------------------------------------------------------
 
 // 64 rows x `tiles_per` column tiles of 128; a warp owns 8 rows, a lane 4 adjacent columns of each.  Bound by the read and
-// write of c, so what a step needs (the tile of c, read and written by the same thread, and up to RC ranks of the adapter)
-// arrives through a two-stage ring of asynchronous copies while the step before it is computed and stored; the rows' t and
-// the row numbers are read once per CTA.  More than RC ranks take several steps per column tile.
+// write of c: the tile of c (64 x 128, read and written by the same thread) and up to RC ranks of the adapter arrive in
+// two-stage rings while the step before is computed and stored; the rows' t and the row numbers are read once per CTA.  t is
+// kept twice, side by side, so that a packed multiply-add takes two columns.  More than RC ranks take several steps per
+// column tile.
 struct ExpandParams {
     Groups g;
     const float* t;       // (rows, rank)
@@ -295,18 +356,17 @@ struct ExpandParams {
     const float* scale;   // (count) or null
     float* c;             // (rows, J)
     int rows, J, rank, act, tiles_per;
-    int w_vec, c_vec;
 };
 
 constexpr int EN = 128;
 
 template <int RC>
 struct ExpandCfg {
-    static constexpr int STAGES = 2, LD = EN + 4, C_FLOATS = TM * EN, STAGE_FLOATS = C_FLOATS + RC * LD;
-    static int smem_bytes(int rank) { return (STAGES * STAGE_FLOATS + TM * ((rank + RC - 1) / RC * RC)) * 4; }
+    static constexpr int LD = EN + 4, C_FLOATS = TM * EN, W_FLOATS = RC * LD;
+    static int smem_bytes(int rank) { return (2 * (C_FLOATS + W_FLOATS) + 2 * TM * rank) * 4; }
 };
 
-template <int RC, bool RMAJ>
+template <int RC, bool RMAJ, bool VEC>
 __global__ void __launch_bounds__(THREADS, 2) expand_kernel(const ExpandParams p)
 {
     using C = ExpandCfg<RC>;
@@ -315,108 +375,125 @@ __global__ void __launch_bounds__(THREADS, 2) expand_kernel(const ExpandParams p
     const Tile tile = tile_of(p.g, blockIdx.x, p.rows);
     if (!tile.valid || (tile.adapter < 0 && p.act == 0)) return;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int rchunks = (p.rank + RC - 1) / RC, rpad = rchunks * RC;
-    float* ts = smem + C::STAGES * C::STAGE_FLOATS;          // [TM][rpad], scaled
-    if (tid < TM) row_s[tid] = tid < tile.rows ? (p.g.perm ? __ldg(p.g.perm + tile.first + tid) : tile.first + tid) : -1;
+    const bool with = tile.adapter >= 0;
+    const int rchunks = with ? (p.rank + RC - 1) / RC : 1;
+    float* cring = smem;                                   // [2][TM][EN]
+    float* wring = smem + 2 * C::C_FLOATS;                 // [2][RC][LD]
+    float* ts = wring + 2 * C::W_FLOATS;                   // [rank][TM][2], scaled
+    tile_row_numbers(p.g, tile, row_s);
     __syncthreads();
     const int ct0 = blockIdx.y * p.tiles_per, ct1 = min((p.J + EN - 1) / EN, ct0 + p.tiles_per);
     const int steps = (ct1 - ct0) * rchunks;
-    const float* w = p.w + static_cast<long long>(tile.adapter < 0 ? 0 : tile.adapter) * p.rank * p.J;
-    float* crow[8];
+    const float* w = p.w + static_cast<long long>(with ? tile.adapter : 0) * p.rank * p.J;
+
+    const float* crow[8];                                  // VEC: this lane's columns of its warp's rows
+    if constexpr (VEC) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int m = row_s[warp * 8 + i];
-        crow[i] = m < 0 ? nullptr : p.c + static_cast<long long>(m) * p.J;
+        for (int i = 0; i < 8; i++) {
+            const int m = row_s[warp * 8 + i];
+            crow[i] = p.c + static_cast<long long>(m < 0 ? row_s[0] : m) * p.J + ct0 * EN + lane * 4;
+        }
     }
     const auto issue = [&](int step) {
         if (step < steps) {
-            const int ct = ct0 + step / rchunks, rc = step % rchunks, j0 = ct * EN, r0 = rc * RC;
-            float* cs = smem + (step % C::STAGES) * C::STAGE_FLOATS;
-            float* ws = cs + C::C_FLOATS;
-            if (rc == 0) {                                   // (stays in its stage for this step; kept in registers for the others)
+            const int ct = step / rchunks, rc = step - ct * rchunks, j0 = (ct0 + ct) * EN, r0 = rc * RC;
+            const int jn = min(EN, p.J - j0), rn = with ? min(RC, p.rank - r0) : 0;
+            float* cs = cring + (ct & 1) * C::C_FLOATS;
+            float* ws = wring + (step & 1) * C::W_FLOATS;
+            if constexpr (VEC) {
+                if (lane * 4 < jn) {
+                    if (rc == 0) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int left = crow[i] ? p.J - j0 - lane * 4 : 0;
-                    copy4(cs + (warp * 8 + i) * EN + lane * 4, left > 0 ? crow[i] + j0 + lane * 4 : p.c, left, p.c_vec);
+                        for (int i = 0; i < 8; i++) copy16(cs + (warp * 8 + i) * EN + lane * 4, crow[i] + ct * EN);
+                    }
+                    if constexpr (!RMAJ) {
+#pragma unroll
+                        for (int i = 0; i < RC / 8; i++)
+                            if (warp + 8 * i < rn)
+                                copy16(ws + (warp + 8 * i) * C::LD + lane * 4, w + static_cast<long long>(r0 + warp + 8 * i) * p.J + j0 + lane * 4);
+                    }
                 }
+            } else {
+                if (rc == 0)
+                    for (int q = tid; q < TM * EN; q += THREADS) {
+                        const int m = row_s[q / EN], n = q % EN;
+                        const bool there = m >= 0 && n < jn;
+                        copy1(cs + q, there ? p.c + static_cast<long long>(m) * p.J + j0 + n : p.c, there);
+                    }
+                if (!RMAJ)
+                    for (int q = tid; q < rn * EN; q += THREADS) {
+                        const int r = q / EN, n = q % EN;
+                        copy1(ws + r * C::LD + n, n < jn ? w + static_cast<long long>(r0 + r) * p.J + j0 + n : p.w, n < jn);
+                    }
             }
-            if (tile.adapter >= 0) {
-                if (RMAJ) {
-                    // B is read along its ranks and stored rank by rank
-#pragma unroll 4
-                    for (int q = tid; q < EN * RC; q += THREADS) {
-                        const int n = q / RC, r = q % RC;
-                        const bool there = j0 + n < p.J && r0 + r < p.rank;
-                        copy1(ws + r * C::LD + n, there ? w + static_cast<long long>(j0 + n) * p.rank + r0 + r : p.w, there);
-                    }
-                } else {
-#pragma unroll
-                    for (int q = tid; q < RC * (EN / 4); q += THREADS) {
-                        const int r = q / (EN / 4), n = (q % (EN / 4)) * 4, left = r0 + r < p.rank ? p.J - j0 - n : 0;
-                        copy4(ws + r * C::LD + n, left > 0 ? w + static_cast<long long>(r0 + r) * p.J + j0 + n : p.w, left, p.w_vec);
-                    }
-                }
+            if constexpr (RMAJ) {
+                // B is read along its ranks and stored rank by rank
+                constexpr int NS = THREADS / RC;
+                const int r = tid % RC, n0 = tid / RC;
+                const float* src = w + static_cast<long long>(j0 + n0) * p.rank + r0 + r;
+                float* dst = ws + r * C::LD + n0;
+                const long long hop = static_cast<long long>(NS) * p.rank;
+                const int last = r < rn ? jn : 0;
+#pragma unroll 8
+                for (int n = n0; n < EN; n += NS, src += hop, dst += NS) copy1(dst, n < last ? src : p.w, n < last);
             }
         }
         commit_copies();
     };
     issue(0);
-    if (tile.adapter >= 0) {
+    if (with) {
         const float scale = p.scale ? __ldg(p.scale + tile.adapter) : 1.f;
-        for (int e = tid; e < TM * rpad; e += THREADS) {
-            const int r = e / rpad, c = e - r * rpad;
-            ts[e] = row_s[r] >= 0 && c < p.rank ? scale * __ldg(p.t + static_cast<long long>(row_s[r]) * p.rank + c) : 0.f;
+        for (int e = tid; e < TM * p.rank; e += THREADS) {
+            const int r = e / p.rank, c = e - r * p.rank;
+            const float v = row_s[r] >= 0 ? scale * __ldg(p.t + static_cast<long long>(row_s[r]) * p.rank + c) : 0.f;
+            *reinterpret_cast<float2*>(ts + (c * TM + r) * 2) = make_float2(v, v);
         }
     }
-    float4 cv[8], acc[8];
+    float2 acc[8][2];
     for (int step = 0; step < steps; step++) {
         issue(step + 1);
         wait_copies<1>();
         __syncthreads();
-        const int rc = step % rchunks, j = (ct0 + step / rchunks) * EN + lane * 4, left = p.J - j;
-        const float* cs = smem + (step % C::STAGES) * C::STAGE_FLOATS;
-        const float* ws = cs + C::C_FLOATS;
+        const int ct = step / rchunks, rc = step - ct * rchunks;
+        const float* ws = wring + (step & 1) * C::W_FLOATS + lane * 4;
         if (rc == 0) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                cv[i] = *reinterpret_cast<const float4*>(cs + (warp * 8 + i) * EN + lane * 4);
-                acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            }
+            for (int i = 0; i < 8; i++) acc[i][0] = acc[i][1] = make_float2(0.f, 0.f);
         }
-        if (tile.adapter >= 0) {
+        if (with) {
+            const int rn = min(RC, p.rank - rc * RC);
+            const float* tp = ts + (rc * RC * TM + warp * 8) * 2;
+#pragma unroll 4
+            for (int r = 0; r < rn; r++) {
+                const float4 wv = *reinterpret_cast<const float4*>(ws + r * C::LD);
 #pragma unroll
-            for (int r = 0; r < RC; r += 4) {
-                float4 wv[4];
-#pragma unroll
-                for (int q = 0; q < 4; q++) wv[q] = *reinterpret_cast<const float4*>(ws + (r + q) * C::LD + lane * 4);
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float4 tv = *reinterpret_cast<const float4*>(ts + (warp * 8 + i) * rpad + rc * RC + r);
-                    const float t4[4] = {tv.x, tv.y, tv.z, tv.w};
-#pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        acc[i].x = fmaf(t4[q], wv[q].x, acc[i].x);
-                        acc[i].y = fmaf(t4[q], wv[q].y, acc[i].y);
-                        acc[i].z = fmaf(t4[q], wv[q].z, acc[i].z);
-                        acc[i].w = fmaf(t4[q], wv[q].w, acc[i].w);
-                    }
+                for (int i = 0; i < 8; i += 2) {
+                    const float4 tv = *reinterpret_cast<const float4*>(tp + (r * TM + i) * 2);
+                    acc[i][0] = __ffma2_rn(make_float2(tv.x, tv.y), make_float2(wv.x, wv.y), acc[i][0]);
+                    acc[i][1] = __ffma2_rn(make_float2(tv.x, tv.y), make_float2(wv.z, wv.w), acc[i][1]);
+                    acc[i + 1][0] = __ffma2_rn(make_float2(tv.z, tv.w), make_float2(wv.x, wv.y), acc[i + 1][0]);
+                    acc[i + 1][1] = __ffma2_rn(make_float2(tv.z, tv.w), make_float2(wv.z, wv.w), acc[i + 1][1]);
                 }
             }
         }
         if (rc == rchunks - 1) {
+            const int j = (ct0 + ct) * EN + lane * 4, left = p.J - j;
+            const float* cs = cring + (ct & 1) * C::C_FLOATS + lane * 4;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                if (!crow[i]) continue;
-                float4 v = make_float4(cv[i].x + acc[i].x, cv[i].y + acc[i].y, cv[i].z + acc[i].z, cv[i].w + acc[i].w);
+                const int m = row_s[warp * 8 + i];
+                if (m < 0 || left <= 0) continue;
+                float4 v = *reinterpret_cast<const float4*>(cs + (warp * 8 + i) * EN);
+                v.x += acc[i][0].x; v.y += acc[i][0].y; v.z += acc[i][1].x; v.w += acc[i][1].y;
                 if (p.act) {
                     v.x = act_apply(v.x, p.act); v.y = act_apply(v.y, p.act);
                     v.z = act_apply(v.z, p.act); v.w = act_apply(v.w, p.act);
                 }
-                float* dst = crow[i] + j;
-                if (p.c_vec && left >= 4) {
+                float* dst = p.c + static_cast<long long>(m) * p.J + j;
+                if (VEC) {
                     *reinterpret_cast<float4*>(dst) = v;
                 } else {
-                    if (left > 0) dst[0] = v.x;
+                    dst[0] = v.x;
                     if (left > 1) dst[1] = v.y;
                     if (left > 2) dst[2] = v.z;
                     if (left > 3) dst[3] = v.w;
@@ -425,13 +502,14 @@ __global__ void __launch_bounds__(THREADS, 2) expand_kernel(const ExpandParams p
         }
         __syncthreads();
     }
+    wait_copies<0>();
 }
 
 // ---- outer ----------------------------------------------------------------------------------------
 
-// out = small^T . big over one adapter's rows: a tile of RP ranks x 128 columns.  A thread owns 8 ranks x 4 columns; the
-// 4 RP threads that cover the tile once form a row group, and the row groups of the CTA share out the rows of every
-// chunk of 32, which arrive through a ring of asynchronous copies.  The CTAs of a cluster cut the adapter's rows into
+// out = small^T . big over one adapter's rows: a tile of RP ranks x 128 columns.  A thread owns RT (8, or 16) ranks x 4
+// columns, a packed multiply-add serves two ranks; the 32 RP / RT threads that cover the tile once form a row group, and the
+// row groups of the CTA share out the rows of every chunk of 32.  The CTAs of a cluster cut the adapter's rows into
 // contiguous ranges.  Joins as in shrink_kernel.  Two jobs in one grid: dA (rank, K) from dt and x, dB (N, rank) from t
 // and g.
 struct OuterJob {
@@ -439,7 +517,7 @@ struct OuterJob {
     const float* big;     // (rows, C)
     float* out;           // (count, rank, C), or (count, C, rank) when col_major
     const float* scale;   // (count) or null
-    int C, col_major, tiles, big_vec, small_vec;
+    int C, col_major, tiles;
 };
 
 struct OuterParams {
@@ -451,16 +529,16 @@ struct OuterParams {
 template <int RP>
 struct OuterCfg {
     static constexpr int MC = 32, CN = 128, STAGES = 3, STAGE_FLOATS = MC * CN + MC * RP;
-    static constexpr int RED_FLOATS = THREADS / (4 * RP) * RP * CN;
+    static constexpr int RT = RP < 16 ? RP : 16, GROUP = 32 * (RP / RT), MG = THREADS / GROUP;
+    static constexpr int RED_FLOATS = MG * RP * CN;
     static constexpr int SMEM_BYTES = (STAGES * STAGE_FLOATS > RED_FLOATS ? STAGES * STAGE_FLOATS : RED_FLOATS) * 4;
 };
 
-template <int RP>
-__global__ void __launch_bounds__(THREADS) outer_kernel(const OuterParams p)
+template <int RP, bool VEC>
+__global__ void __launch_bounds__(THREADS, 2) outer_kernel(const OuterParams p)
 {
     using C = OuterCfg<RP>;
-    constexpr int MC = C::MC, CN = C::CN, GROUP = 4 * RP, MG = THREADS / GROUP;
-    constexpr int BL = MC * CN / 4 / THREADS;
+    constexpr int MC = C::MC, CN = C::CN, STAGES = C::STAGES, RT = C::RT, GROUP = C::GROUP, MG = C::MG;
     extern __shared__ __align__(16) float smem[];
     cg::cluster_group cluster = cg::this_cluster();
     const int S = static_cast<int>(cluster.num_blocks()), split = static_cast<int>(cluster.block_rank());
@@ -468,7 +546,7 @@ __global__ void __launch_bounds__(THREADS) outer_kernel(const OuterParams p)
     int ct = blockIdx.x / S;
     const OuterJob& job = p.job[ct < p.job[0].tiles ? 0 : 1];
     if (ct >= p.job[0].tiles) ct -= p.job[0].tiles;
-    const int c0 = ct * CN;
+    const int c0 = ct * CN, cn = min(CN, job.C - c0), rn = min(RP, p.rank - rb);
     int first = 0, n = p.rows;
     if (p.g.perm) {
         first = __ldg(p.g.offset + e);
@@ -480,52 +558,81 @@ __global__ void __launch_bounds__(THREADS) outer_kernel(const OuterParams p)
     const int m0 = split * span, m1 = min(n, m0 + span);
     const int chunks = m1 > m0 ? (m1 - m0 + MC - 1) / MC : 0;
 
+    // VEC: this thread's places of a stage, and the rows of the next fill (a grouping's are looked up a fill ahead)
+    constexpr int BN = MC * CN / 4 / THREADS, Q = RP / 4, SN = (MC * Q + THREADS - 1) / THREADS;
+    const int c4 = (tid % 32) * 4, br = tid / 32, s4 = (tid % Q) * 4, sr = tid / Q;
+    int brow[BN], srow[SN];
+    const auto look_up = [&](int chunk) {
+        const int m = m0 + chunk * MC;
+#pragma unroll
+        for (int i = 0; i < BN; i++) brow[i] = p.g.perm ? __ldg(p.g.perm + first + min(m + br + 8 * i, m1 - 1)) : min(m + br + 8 * i, m1 - 1);
+#pragma unroll
+        for (int i = 0; i < SN; i++) {
+            const int r = min(m + sr + i * (THREADS / Q), m1 - 1);
+            srow[i] = p.g.perm ? __ldg(p.g.perm + first + r) : r;
+        }
+    };
     const auto issue = [&](int chunk) {
         if (chunk < chunks) {
-            float* bs = smem + (chunk % C::STAGES) * C::STAGE_FLOATS;
+            float* bs = smem + (chunk % STAGES) * C::STAGE_FLOATS;
             float* ss = bs + MC * CN;
-            const int m = m0 + chunk * MC;
-            const int cl = (tid % (CN / 4)) * 4;
+            const int m = m0 + chunk * MC, mn = min(MC, m1 - m);
+            if constexpr (VEC) {
+                if (c4 < cn) {
 #pragma unroll
-            for (int i = 0; i < BL; i++) {
-                const int r = tid / (CN / 4) + i * (THREADS / (CN / 4));
-                const int left = m + r < m1 ? job.C - c0 - cl : 0;
-                const long long row = left > 0 ? (p.g.perm ? __ldg(p.g.perm + first + m + r) : m + r) : 0;
-                copy4(bs + r * CN + cl, left > 0 ? job.big + row * job.C + c0 + cl : job.big, left, job.big_vec);
-            }
+                    for (int i = 0; i < BN; i++) copy16(bs + (br + 8 * i) * CN + c4, job.big + static_cast<long long>(brow[i]) * job.C + c0 + c4);
+                }
+                if (s4 < rn && (MC * Q >= THREADS || sr < MC)) {
 #pragma unroll
-            for (int q = tid; q < MC * RP / 4; q += THREADS) {
-                const int r = q / (RP / 4), c = rb + (q % (RP / 4)) * 4;
-                const int left = m + r < m1 ? p.rank - c : 0;
-                const long long row = left > 0 ? (p.g.perm ? __ldg(p.g.perm + first + m + r) : m + r) : 0;
-                copy4(ss + q * 4, left > 0 ? job.small + row * p.rank + c : job.small, left, job.small_vec);
+                    for (int i = 0; i < SN; i++)
+                        copy16(ss + (sr + i * (THREADS / Q)) * RP + s4, job.small + static_cast<long long>(srow[i]) * p.rank + rb + s4);
+                }
+                if (chunk + 1 < chunks) look_up(chunk + 1);
+            } else {
+                for (int q = tid; q < mn * CN; q += THREADS) {
+                    const int r = q / CN, c = q % CN;
+                    const long long row = p.g.perm ? __ldg(p.g.perm + first + m + r) : m + r;
+                    copy1(bs + q, c < cn ? job.big + row * job.C + c0 + c : job.big, c < cn);
+                }
+                for (int q = tid; q < mn * RP; q += THREADS) {
+                    const int r = q / RP, c = q % RP;
+                    const long long row = p.g.perm ? __ldg(p.g.perm + first + m + r) : m + r;
+                    copy1(ss + q, c < rn ? job.small + row * p.rank + rb + c : job.small, c < rn);
+                }
             }
         }
         commit_copies();
     };
-    const int mg = tid / GROUP, t = tid % GROUP, cl = t % 32, rg = t / 32;   // rg: 8 ranks, cl: 4 columns
-    float4 acc[8];
+    if (VEC && chunks > 0) look_up(0);
+    const int mg = tid / GROUP, t = tid % GROUP, cl = t % 32, rg = t / 32;   // rg: RT ranks, cl: 4 columns
+    float2 acc[RT / 2][4];                                                   // [rank pair][column]
 #pragma unroll
-    for (int i = 0; i < 8; i++) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < C::STAGES - 1; s++) issue(s);
-    for (int chunk = 0; chunk < chunks; chunk++) {
-        wait_copies<C::STAGES - 2>();
+    for (int i = 0; i < RT / 2; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) acc[i][j] = make_float2(0.f, 0.f);
+    for (int s = 0; s < STAGES - 1; s++) issue(s);
+    for (int done = 0; done < chunks; done++) {
+        wait_copies<STAGES - 2>();
         __syncthreads();
-        issue(chunk + C::STAGES - 1);
-        const float* bs = smem + (chunk % C::STAGES) * C::STAGE_FLOATS;
-        const float* ss = bs + MC * CN;
-#pragma unroll 4
-        for (int r = mg; r < MC; r += MG) {
-            const float4 bv = *reinterpret_cast<const float4*>(bs + r * CN + cl * 4);
-            float sv[8];
-            *reinterpret_cast<float4*>(sv) = *reinterpret_cast<const float4*>(ss + r * RP + rg * 8);
-            *reinterpret_cast<float4*>(sv + 4) = *reinterpret_cast<const float4*>(ss + r * RP + rg * 8 + 4);
+        issue(done + STAGES - 1);
+        const float* bs = smem + (done % STAGES) * C::STAGE_FLOATS + cl * 4;
+        const float* ss = smem + (done % STAGES) * C::STAGE_FLOATS + MC * CN + rg * RT;
+        const int mn = min(MC, m1 - m0 - done * MC);
+#pragma unroll 2
+        for (int r = mg; r < mn; r += MG) {
+            const float4 bv = *reinterpret_cast<const float4*>(bs + r * CN);
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                acc[i].x = fmaf(sv[i], bv.x, acc[i].x);
-                acc[i].y = fmaf(sv[i], bv.y, acc[i].y);
-                acc[i].z = fmaf(sv[i], bv.z, acc[i].z);
-                acc[i].w = fmaf(sv[i], bv.w, acc[i].w);
+            for (int i = 0; i < RT / 4; i++) {
+                const float4 sv = *reinterpret_cast<const float4*>(ss + r * RP + 4 * i);
+                const float2 s0 = make_float2(sv.x, sv.y), s1 = make_float2(sv.z, sv.w);
+                acc[2 * i][0] = __ffma2_rn(s0, make_float2(bv.x, bv.x), acc[2 * i][0]);
+                acc[2 * i][1] = __ffma2_rn(s0, make_float2(bv.y, bv.y), acc[2 * i][1]);
+                acc[2 * i][2] = __ffma2_rn(s0, make_float2(bv.z, bv.z), acc[2 * i][2]);
+                acc[2 * i][3] = __ffma2_rn(s0, make_float2(bv.w, bv.w), acc[2 * i][3]);
+                acc[2 * i + 1][0] = __ffma2_rn(s1, make_float2(bv.x, bv.x), acc[2 * i + 1][0]);
+                acc[2 * i + 1][1] = __ffma2_rn(s1, make_float2(bv.y, bv.y), acc[2 * i + 1][1]);
+                acc[2 * i + 1][2] = __ffma2_rn(s1, make_float2(bv.z, bv.z), acc[2 * i + 1][2]);
+                acc[2 * i + 1][3] = __ffma2_rn(s1, make_float2(bv.w, bv.w), acc[2 * i + 1][3]);
             }
         }
     }
@@ -533,7 +640,11 @@ __global__ void __launch_bounds__(THREADS) outer_kernel(const OuterParams p)
     __syncthreads();
     // partial tiles [mg][rank][column]
 #pragma unroll
-    for (int i = 0; i < 8; i++) *reinterpret_cast<float4*>(smem + (mg * RP + rg * 8 + i) * CN + cl * 4) = acc[i];
+    for (int i = 0; i < RT / 2; i++) {
+        float* dst = smem + (mg * RP + rg * RT + 2 * i) * CN + cl * 4;
+        *reinterpret_cast<float4*>(dst) = make_float4(acc[i][0].x, acc[i][1].x, acc[i][2].x, acc[i][3].x);
+        *reinterpret_cast<float4*>(dst + CN) = make_float4(acc[i][0].y, acc[i][1].y, acc[i][2].y, acc[i][3].y);
+    }
     __syncthreads();
     if (MG > 1) {
         for (int q = tid; q < RP * CN; q += THREADS) {
@@ -551,7 +662,7 @@ __global__ void __launch_bounds__(THREADS) outer_kernel(const OuterParams p)
         const int k = split * per + q;
         // neighbouring threads write neighbouring addresses in either layout
         const int r = job.col_major ? k % RP : k / CN, c = job.col_major ? k / RP : k % CN;
-        if (rb + r >= p.rank || c0 + c >= job.C) continue;
+        if (r >= rn || c >= cn) continue;
         float s = S > 1 ? *cluster.map_shared_rank(smem + r * CN + c, 0) : smem[r * CN + c];
         for (int o = 1; o < S; o++) s += *cluster.map_shared_rank(smem + r * CN + c, o);
         out[job.col_major ? static_cast<long long>(c0 + c) * p.rank + rb + r : static_cast<long long>(rb + r) * job.C + c0 + c] = scale * s;
@@ -586,6 +697,76 @@ int tile_bound(int rows, int adapters)
     return rows / TM + groups;
 }
 
+// Clusters of a launch: doubled while the CTAs still fit the SMs once, two on each, and `longest` leaves enough work per CTA.
+int cluster_size(long long ctas, int longest, int least, int num_sms)
+{
+    int S = 1;
+    while (S < 8 && ctas * S * 2 <= 2ll * num_sms && longest / (2 * S) >= least) S *= 2;
+    return S;
+}
+
+template <int RP, bool KMAJ>
+cudaError_t launch_shrink_t(cudaStream_t st, const ShrinkParams& p, int tiles, bool vec, int num_sms)
+{
+    const int rblocks = (p.rank + RP - 1) / RP;
+    const int S = cluster_size(static_cast<long long>(tiles) * rblocks, p.L, 2 * ShrinkCfg<RP, KMAJ>::KC, num_sms);
+    const dim3 grid(static_cast<unsigned int>(tiles) * S, rblocks, 1);
+    const int smem = ShrinkCfg<RP, KMAJ>::smem_bytes(p.rank);
+    return vec ? launch_cluster(st, shrink_kernel<RP, KMAJ, true>, grid, S, smem, p)
+                : launch_cluster(st, shrink_kernel<RP, KMAJ, false>, grid, S, smem, p);
+}
+
+template <int RC, bool RMAJ>
+cudaError_t launch_expand_t(cudaStream_t st, const ExpandParams& p, dim3 grid, bool vec)
+{
+    const int smem = ExpandCfg<RC>::smem_bytes(p.rank);
+    if (vec) expand_kernel<RC, RMAJ, true><<<grid, THREADS, smem, st>>>(p);
+    else      expand_kernel<RC, RMAJ, false><<<grid, THREADS, smem, st>>>(p);
+    return cudaGetLastError();
+}
+
+template <int RP>
+cudaError_t launch_outer_t(cudaStream_t st, const OuterParams& p, int groups, int count, bool vec, int num_sms)
+{
+    const int tiles = p.job[0].tiles + p.job[1].tiles, rblocks = (p.rank + RP - 1) / RP;
+    const int S = cluster_size(static_cast<long long>(tiles) * rblocks * groups, p.rows / groups, 2 * OuterCfg<RP>::MC, num_sms);
+    // (without a grouping the adapters behind the first have no rows: their CTAs store zeros)
+    const dim3 grid(static_cast<unsigned int>(tiles) * S, count, rblocks);
+    return vec ? launch_cluster(st, outer_kernel<RP, true>, grid, S, OuterCfg<RP>::SMEM_BYTES, p)
+                : launch_cluster(st, outer_kernel<RP, false>, grid, S, OuterCfg<RP>::SMEM_BYTES, p);
+}
+
+template <typename K>
+cudaError_t allow_smem(K* kernel, int bytes) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); }
+
+template <int RP, bool VEC>
+cudaError_t init_rank()
+{
+    const int most = RP == 64 ? MAX_RANK : RP;
+    cudaError_t e;
+    if ((e = allow_smem(shrink_kernel<RP, true, VEC>, ShrinkCfg<RP, true>::smem_bytes(most))) != cudaSuccess) return e;
+    if ((e = allow_smem(shrink_kernel<RP, false, VEC>, ShrinkCfg<RP, false>::smem_bytes(most))) != cudaSuccess) return e;
+    return allow_smem(outer_kernel<RP, VEC>, OuterCfg<RP>::SMEM_BYTES);
+}
+
+template <int RC, bool VEC>
+cudaError_t init_expand()
+{
+    const int bytes = ExpandCfg<RC>::smem_bytes(RC == 32 ? MAX_RANK : RC);
+    const cudaError_t e = allow_smem(expand_kernel<RC, true, VEC>, bytes);
+    return e != cudaSuccess ? e : allow_smem(expand_kernel<RC, false, VEC>, bytes);
+}
+
+template <bool VEC>
+cudaError_t init_vec()
+{
+    cudaError_t e;
+    if ((e = init_rank<8, VEC>()) != cudaSuccess || (e = init_rank<16, VEC>()) != cudaSuccess || (e = init_rank<32, VEC>()) != cudaSuccess ||
+        (e = init_rank<64, VEC>()) != cudaSuccess || (e = init_expand<8, VEC>()) != cudaSuccess || (e = init_expand<16, VEC>()) != cudaSuccess)
+        return e;
+    return init_expand<32, VEC>();
+}
+
 }  // namespace
 
 size_t groups_bytes(int rows, int adapters)
@@ -618,6 +799,12 @@ cudaError_t launch_group(cudaStream_t st, const Groups& g, const int* row_adapte
     return cudaGetLastError();
 }
 
+cudaError_t init_tiled()
+{
+    const cudaError_t e = init_vec<true>();
+    return e != cudaSuccess ? e : init_vec<false>();
+}
+
 cudaError_t launch_shrink(cudaStream_t st, const Groups& g, const Adapters& ad, bool down, bool scaled, const float* x,
                           float* out, int rows, int L, int num_sms)
 {
@@ -628,24 +815,18 @@ cudaError_t launch_shrink(cudaStream_t st, const Groups& g, const Adapters& ad, 
     p.scale = scaled ? ad.scale : nullptr;
     p.out = out;
     p.rows = rows; p.L = L; p.rank = ad.rank;
-    p.x_vec = aligned16(x) && L % 4 == 0;
-    p.w_vec = down && aligned16(p.w) && L % 4 == 0;
+    const bool vec = L % 4 == 0 && aligned16(x) && aligned16(p.w) && (down || ad.rank % 4 == 0);
     const int tiles = g.perm ? g.max_tiles : (rows + TM - 1) / TM;
-    const int rp = ad.rank <= 8 ? 8 : ad.rank <= 16 ? 16 : ad.rank <= 32 ? 32 : 64;
-    const int rblocks = (ad.rank + rp - 1) / rp;
-    int S = 1;
-    while (S < 8 && static_cast<long long>(tiles) * rblocks * S < 3ll * num_sms && L / (2 * S) >= 64) S *= 2;
-    const dim3 grid(static_cast<unsigned int>(tiles) * S, rblocks, 1);
     if (down) {
-        if (rp == 8)       return launch_cluster(st, shrink_kernel<8, true>, grid, S, ShrinkCfg<8>::SMEM_BYTES, p);
-        else if (rp == 16) return launch_cluster(st, shrink_kernel<16, true>, grid, S, ShrinkCfg<16>::SMEM_BYTES, p);
-        else if (rp == 32) return launch_cluster(st, shrink_kernel<32, true>, grid, S, ShrinkCfg<32>::SMEM_BYTES, p);
-        return launch_cluster(st, shrink_kernel<64, true>, grid, S, ShrinkCfg<64>::SMEM_BYTES, p);
+        if (ad.rank <= 8)  return launch_shrink_t<8, true>(st, p, tiles, vec, num_sms);
+        if (ad.rank <= 16) return launch_shrink_t<16, true>(st, p, tiles, vec, num_sms);
+        if (ad.rank <= 32) return launch_shrink_t<32, true>(st, p, tiles, vec, num_sms);
+        return launch_shrink_t<64, true>(st, p, tiles, vec, num_sms);
     }
-    if (rp == 8)       return launch_cluster(st, shrink_kernel<8, false>, grid, S, ShrinkCfg<8>::SMEM_BYTES, p);
-    else if (rp == 16) return launch_cluster(st, shrink_kernel<16, false>, grid, S, ShrinkCfg<16>::SMEM_BYTES, p);
-    else if (rp == 32) return launch_cluster(st, shrink_kernel<32, false>, grid, S, ShrinkCfg<32>::SMEM_BYTES, p);
-    return launch_cluster(st, shrink_kernel<64, false>, grid, S, ShrinkCfg<64>::SMEM_BYTES, p);
+    if (ad.rank <= 8)  return launch_shrink_t<8, false>(st, p, tiles, vec, num_sms);
+    if (ad.rank <= 16) return launch_shrink_t<16, false>(st, p, tiles, vec, num_sms);
+    if (ad.rank <= 32) return launch_shrink_t<32, false>(st, p, tiles, vec, num_sms);
+    return launch_shrink_t<64, false>(st, p, tiles, vec, num_sms);
 }
 
 cudaError_t launch_expand(cudaStream_t st, const Groups& g, const Adapters& ad, bool up, bool scaled, const float* t,
@@ -658,24 +839,20 @@ cudaError_t launch_expand(cudaStream_t st, const Groups& g, const Adapters& ad, 
     p.scale = scaled ? ad.scale : nullptr;
     p.c = c;
     p.rows = rows; p.J = J; p.rank = ad.rank; p.act = act;
-    p.w_vec = !up && aligned16(p.w) && J % 4 == 0;
-    p.c_vec = aligned16(c) && J % 4 == 0;
+    const bool vec = J % 4 == 0 && aligned16(c) && (up || aligned16(p.w));
     const int tiles = g.perm ? g.max_tiles : (rows + TM - 1) / TM, cols = (J + EN - 1) / EN;
     // column tiles per CTA: as many as leave four CTAs per SM
-    long long per = static_cast<long long>(tiles) * cols / (4ll * num_sms);
+    const long long per = static_cast<long long>(tiles) * cols / (4ll * num_sms);
     p.tiles_per = static_cast<int>(per < 1 ? 1 : per > 8 ? 8 : per);
     const dim3 grid(tiles, (cols + p.tiles_per - 1) / p.tiles_per, 1);
-    const int rc = ad.rank <= 8 ? 8 : ad.rank <= 16 ? 16 : 32;
     if (up) {
-        if (rc == 8)       expand_kernel<8, true><<<grid, THREADS, ExpandCfg<8>::smem_bytes(ad.rank), st>>>(p);
-        else if (rc == 16) expand_kernel<16, true><<<grid, THREADS, ExpandCfg<16>::smem_bytes(ad.rank), st>>>(p);
-        else               expand_kernel<32, true><<<grid, THREADS, ExpandCfg<32>::smem_bytes(ad.rank), st>>>(p);
-    } else {
-        if (rc == 8)       expand_kernel<8, false><<<grid, THREADS, ExpandCfg<8>::smem_bytes(ad.rank), st>>>(p);
-        else if (rc == 16) expand_kernel<16, false><<<grid, THREADS, ExpandCfg<16>::smem_bytes(ad.rank), st>>>(p);
-        else               expand_kernel<32, false><<<grid, THREADS, ExpandCfg<32>::smem_bytes(ad.rank), st>>>(p);
+        if (ad.rank <= 8)  return launch_expand_t<8, true>(st, p, grid, vec);
+        if (ad.rank <= 16) return launch_expand_t<16, true>(st, p, grid, vec);
+        return launch_expand_t<32, true>(st, p, grid, vec);
     }
-    return cudaGetLastError();
+    if (ad.rank <= 8)  return launch_expand_t<8, false>(st, p, grid, vec);
+    if (ad.rank <= 16) return launch_expand_t<16, false>(st, p, grid, vec);
+    return launch_expand_t<32, false>(st, p, grid, vec);
 }
 
 cudaError_t launch_outer(cudaStream_t st, const Groups& g, const Adapters& ad, const float* dt, const float* x, float* da,
@@ -687,53 +864,22 @@ cudaError_t launch_outer(cudaStream_t st, const Groups& g, const Adapters& ad, c
     p.rank = ad.rank;
     int jobs = 0;
     p.job[0].tiles = p.job[1].tiles = 0;
-    if (da) p.job[jobs++] = OuterJob{dt, x, da, nullptr, K, 0, (K + 127) / 128, aligned16(x) && K % 4 == 0, aligned16(dt) && ad.rank % 4 == 0};
-    if (db) p.job[jobs++] = OuterJob{t, grad, db, ad.scale, N, 1, (N + 127) / 128, aligned16(grad) && N % 4 == 0, aligned16(t) && ad.rank % 4 == 0};
+    bool vec = ad.rank % 4 == 0;
+    if (da) {
+        p.job[jobs++] = OuterJob{dt, x, da, nullptr, K, 0, (K + 127) / 128};
+        vec = vec && K % 4 == 0 && aligned16(x) && aligned16(dt);
+    }
+    if (db) {
+        p.job[jobs++] = OuterJob{t, grad, db, ad.scale, N, 1, (N + 127) / 128};
+        vec = vec && N % 4 == 0 && aligned16(grad) && aligned16(t);
+    }
     if (jobs == 0) return cudaSuccess;
     if (jobs == 1) { p.job[1] = p.job[0]; p.job[1].tiles = 0; }
-    const int rp = ad.rank <= 8 ? 8 : ad.rank <= 16 ? 16 : ad.rank <= 32 ? 32 : 64;
-    const int rblocks = (ad.rank + rp - 1) / rp;
-    const int tiles = p.job[0].tiles + p.job[1].tiles;
     const int groups = g.perm ? ad.count : 1;
-    int S = 1;
-    while (S < 8 && static_cast<long long>(tiles) * rblocks * groups * S < 3ll * num_sms && rows / (2 * S * groups) >= 32) S *= 2;
-    // (without a grouping the adapters behind the first have no rows: their CTAs store zeros)
-    const dim3 grid(static_cast<unsigned int>(tiles) * S, ad.count, rblocks);
-    if (rp == 8)       return launch_cluster(st, outer_kernel<8>, grid, S, OuterCfg<8>::SMEM_BYTES, p);
-    else if (rp == 16) return launch_cluster(st, outer_kernel<16>, grid, S, OuterCfg<16>::SMEM_BYTES, p);
-    else if (rp == 32) return launch_cluster(st, outer_kernel<32>, grid, S, OuterCfg<32>::SMEM_BYTES, p);
-    return launch_cluster(st, outer_kernel<64>, grid, S, OuterCfg<64>::SMEM_BYTES, p);
-}
-
-namespace {
-template <typename K>
-cudaError_t allow_smem(K* kernel, int bytes) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); }
-
-template <int RP>
-cudaError_t init_rank()
-{
-    cudaError_t e;
-    if ((e = allow_smem(shrink_kernel<RP, true>, ShrinkCfg<RP>::SMEM_BYTES)) != cudaSuccess) return e;
-    if ((e = allow_smem(shrink_kernel<RP, false>, ShrinkCfg<RP>::SMEM_BYTES)) != cudaSuccess) return e;
-    return allow_smem(outer_kernel<RP>, OuterCfg<RP>::SMEM_BYTES);
-}
-
-template <int RC>
-cudaError_t init_expand()
-{
-    const int bytes = ExpandCfg<RC>::smem_bytes(RC == 32 ? MAX_RANK : RC);
-    const cudaError_t e = allow_smem(expand_kernel<RC, true>, bytes);
-    return e != cudaSuccess ? e : allow_smem(expand_kernel<RC, false>, bytes);
-}
-}  // namespace
-
-cudaError_t init_tiled()
-{
-    cudaError_t e;
-    if ((e = init_rank<8>()) != cudaSuccess || (e = init_rank<16>()) != cudaSuccess || (e = init_rank<32>()) != cudaSuccess ||
-        (e = init_rank<64>()) != cudaSuccess || (e = init_expand<8>()) != cudaSuccess || (e = init_expand<16>()) != cudaSuccess)
-        return e;
-    return init_expand<32>();
+    if (ad.rank <= 8)  return launch_outer_t<8>(st, p, groups, ad.count, vec, num_sms);
+    if (ad.rank <= 16) return launch_outer_t<16>(st, p, groups, ad.count, vec, num_sms);
+    if (ad.rank <= 32) return launch_outer_t<32>(st, p, groups, ad.count, vec, num_sms);
+    return launch_outer_t<64>(st, p, groups, ad.count, vec, num_sms);
 }
 
 }  // namespace lora

@@ -33,6 +33,12 @@ __device__ __forceinline__ void copy4(float* dst, const float* src, int n, bool 
     }
 }
 
+// Sixteen bytes, all there.
+__device__ __forceinline__ void copy16(float* dst, const float* src)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+
 __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
 // Waits until at most N of the calling thread's copy groups are unfinished.
