@@ -160,7 +160,7 @@ __device__ __forceinline__ void tile_row_numbers(const Groups& g, const Tile& ti
 // ---- shrink ---------------------------------------------------------------------------------------
 
 // A tile of 64 rows x RP ranks.  A thread owns 4 rows x 8 ranks; the 2 RP threads that cover the tile once form a k group,
-// and the 128 / RP k groups of the CTA share out the contraction index of every chunk of 64.  KMAJ: both operands
+// and the 128 / RP k groups of the CTA share out the contraction index of every chunk of 128.  KMAJ: both operands
 // have the contraction index contiguous, a 128-bit load of each makes two packed multiply-adds per output (sums over even
 // and odd indices, added at the end); otherwise the ranks are contiguous and a packed multiply-add serves two of them.  The
 // CTAs of a cluster cut the contraction into contiguous ranges; k groups are added through shared memory, the cluster's
@@ -176,7 +176,7 @@ struct ShrinkParams {
 
 template <int RP, bool KMAJ>
 struct ShrinkCfg {
-    static constexpr int KC = 64, LD = KC + 4, STAGES = 4, X_FLOATS = TM * LD;
+    static constexpr int KC = 128, LD = KC + 4, STAGES = 2, X_FLOATS = TM * LD;
     static constexpr int RED_FLOATS = 128 / RP * TM * RP;
     // row pitch of the adapter's part of a stage, and its floats (ranks behind the last one are read past a row's end)
     __host__ __device__ static int pitch(int rank) { return KMAJ ? LD : (rank + 3) & ~3; }
@@ -213,19 +213,15 @@ __global__ void __launch_bounds__(THREADS, 2) shrink_kernel(const ShrinkParams p
     // VEC: this thread's places of a stage
     constexpr int Q = KC / 4, XN = TM * Q / THREADS, WN = (RP * Q + THREADS - 1) / THREADS;
     const int c4 = (tid % Q) * 4, xr = tid / Q;
-    const float* xsrc[XN];
-    const float* wsrc[WN];
+    int xat[XN], wat[WN];                      // (element offsets: int32 reaches every element of x and of one adapter)
     if constexpr (VEC) {
 #pragma unroll
         for (int i = 0; i < XN; i++) {
             const int r = row_s[xr + i * (THREADS / Q)];
-            xsrc[i] = p.x + static_cast<long long>(r < 0 ? row_s[0] : r) * p.L + l0 + c4;
+            xat[i] = (r < 0 ? row_s[0] : r) * p.L + l0 + c4;
         }
 #pragma unroll
-        for (int i = 0; i < WN; i++) {
-            if constexpr (KMAJ) wsrc[i] = w + static_cast<long long>(rb + min(xr + i * (THREADS / Q), wrows - 1)) * p.L + l0 + c4;
-            else                wsrc[i] = w + static_cast<long long>(l0) * p.rank + (tid + i * THREADS) * 4;
-        }
+        for (int i = 0; i < WN; i++) wat[i] = KMAJ ? (rb + min(xr + i * (THREADS / Q), wrows - 1)) * p.L + l0 + c4 : l0 * p.rank + tid * 4;
     }
     const auto issue = [&](int chunk) {
         if (chunk < chunks) {
@@ -235,18 +231,18 @@ __global__ void __launch_bounds__(THREADS, 2) shrink_kernel(const ShrinkParams p
             if constexpr (VEC) {
                 if (c4 < kn) {
 #pragma unroll
-                    for (int i = 0; i < XN; i++) copy16(xs + (xr + i * (THREADS / Q)) * LD + c4, xsrc[i] + chunk * KC);
+                    for (int i = 0; i < XN; i++) copy16(xs + (xr + i * (THREADS / Q)) * LD + c4, p.x + xat[i] + chunk * KC);
                     if constexpr (KMAJ) {
 #pragma unroll
                         for (int i = 0; i < WN; i++)
-                            if (RP * Q >= THREADS || xr < RP) copy16(ws + (xr + i * (THREADS / Q)) * LD + c4, wsrc[i] + chunk * KC);
+                            if (RP * Q >= THREADS || xr < RP) copy16(ws + (xr + i * (THREADS / Q)) * LD + c4, w + wat[i] + chunk * KC);
                     }
                 }
                 if constexpr (!KMAJ) {
                     // (all ranks of kn steps: one dense block)
                     const int n4 = kn * p.rank / 4;
-                    const long long at = static_cast<long long>(chunk) * KC * p.rank;
-                    for (int q = tid, i = 0; q < n4; q += THREADS, i++) copy16(ws + q * 4, wsrc[0] + at + i * (THREADS * 4));
+                    const float* src = w + wat[0] + chunk * KC * p.rank;
+                    for (int q = tid; q < n4; q += THREADS, src += THREADS * 4) copy16(ws + q * 4, src);
                 }
             } else {
                 for (int q = tid; q < TM * KC; q += THREADS) {
@@ -345,10 +341,9 @@ __global__ void __launch_bounds__(THREADS, 2) shrink_kernel(const ShrinkParams p
 // ---- expand ---------------------------------------------------------------------------------------
 
 // 64 rows x `tiles_per` column tiles of 128; a warp owns 8 rows, a lane 4 adjacent columns of each.  Bound by the read and
-// write of c: the tile of c (64 x 128, read and written by the same thread) and up to RC ranks of the adapter arrive in
-// two-stage rings while the step before is computed and stored; the rows' t and the row numbers are read once per CTA.  t is
-// kept twice, side by side, so that a packed multiply-add takes two columns.  More than RC ranks take several steps per
-// column tile.
+// write of c: a step (up to RC ranks of one column tile) asks for its part of c and for the adapter's ranks of the next
+// step, then computes, then adds c, which the same thread asked for and stores, so that c takes one buffer and no
+// barrier.  The rows' t are read once per CTA and kept rank by rank: a packed multiply-add takes two rows.
 struct ExpandParams {
     Groups g;
     const float* t;       // (rows, rank)
@@ -363,11 +358,11 @@ constexpr int EN = 128;
 template <int RC>
 struct ExpandCfg {
     static constexpr int LD = EN + 4, C_FLOATS = TM * EN, W_FLOATS = RC * LD;
-    static int smem_bytes(int rank) { return (2 * (C_FLOATS + W_FLOATS) + 2 * TM * rank) * 4; }
+    static int smem_bytes(int rank) { return (C_FLOATS + 2 * W_FLOATS + TM * rank) * 4; }
 };
 
 template <int RC, bool RMAJ, bool VEC>
-__global__ void __launch_bounds__(THREADS, 2) expand_kernel(const ExpandParams p)
+__global__ void __launch_bounds__(THREADS, 3) expand_kernel(const ExpandParams p)
 {
     using C = ExpandCfg<RC>;
     extern __shared__ __align__(16) float smem[];
@@ -377,54 +372,57 @@ __global__ void __launch_bounds__(THREADS, 2) expand_kernel(const ExpandParams p
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const bool with = tile.adapter >= 0;
     const int rchunks = with ? (p.rank + RC - 1) / RC : 1;
-    float* cring = smem;                                   // [2][TM][EN]
-    float* wring = smem + 2 * C::C_FLOATS;                 // [2][RC][LD]
-    float* ts = wring + 2 * C::W_FLOATS;                   // [rank][TM][2], scaled
+    float* cs = smem;                                      // [TM][EN]
+    float* wring = smem + C::C_FLOATS;                     // [2][RC][LD]
+    float* ts = wring + 2 * C::W_FLOATS;                   // [rank][TM], scaled
     tile_row_numbers(p.g, tile, row_s);
     __syncthreads();
     const int ct0 = blockIdx.y * p.tiles_per, ct1 = min((p.J + EN - 1) / EN, ct0 + p.tiles_per);
     const int steps = (ct1 - ct0) * rchunks;
     const float* w = p.w + static_cast<long long>(with ? tile.adapter : 0) * p.rank * p.J;
 
-    const float* crow[8];                                  // VEC: this lane's columns of its warp's rows
+    int cat[8];                                            // VEC: element offsets of this lane's columns of its warp's rows
     if constexpr (VEC) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const int m = row_s[warp * 8 + i];
-            crow[i] = p.c + static_cast<long long>(m < 0 ? row_s[0] : m) * p.J + ct0 * EN + lane * 4;
+            cat[i] = (m < 0 ? row_s[0] : m) * p.J + ct0 * EN + lane * 4;
         }
     }
-    const auto issue = [&](int step) {
-        if (step < steps) {
-            const int ct = step / rchunks, rc = step - ct * rchunks, j0 = (ct0 + ct) * EN, r0 = rc * RC;
-            const int jn = min(EN, p.J - j0), rn = with ? min(RC, p.rank - r0) : 0;
-            float* cs = cring + (ct & 1) * C::C_FLOATS;
-            float* ws = wring + (step & 1) * C::W_FLOATS;
-            if constexpr (VEC) {
-                if (lane * 4 < jn) {
-                    if (rc == 0) {
+    const auto issue_c = [&](int ct) {
+        const int j0 = (ct0 + ct) * EN, jn = min(EN, p.J - j0);
+        if constexpr (VEC) {
+            if (lane * 4 < jn) {
 #pragma unroll
-                        for (int i = 0; i < 8; i++) copy16(cs + (warp * 8 + i) * EN + lane * 4, crow[i] + ct * EN);
-                    }
-                    if constexpr (!RMAJ) {
+                for (int i = 0; i < 8; i++) copy16(cs + (warp * 8 + i) * EN + lane * 4, p.c + cat[i] + ct * EN);
+            }
+        } else {
+            for (int i = 0; i < 8; i++) {
+                const int m = row_s[warp * 8 + i];
+                copy4(cs + (warp * 8 + i) * EN + lane * 4, m >= 0 && lane * 4 < jn ? p.c + static_cast<long long>(m) * p.J + j0 + lane * 4 : p.c,
+                      m >= 0 ? jn - lane * 4 : 0, false);
+            }
+        }
+    };
+    const auto issue_w = [&](int step) {
+        if (step < steps && with) {
+            const int ct = step / rchunks, rc = step - ct * rchunks, j0 = (ct0 + ct) * EN, r0 = rc * RC;
+            const int jn = min(EN, p.J - j0), rn = min(RC, p.rank - r0);
+            float* ws = wring + (step & 1) * C::W_FLOATS;
+            if constexpr (!RMAJ) {
+                if constexpr (VEC) {
+                    if (lane * 4 < jn) {
 #pragma unroll
                         for (int i = 0; i < RC / 8; i++)
                             if (warp + 8 * i < rn)
                                 copy16(ws + (warp + 8 * i) * C::LD + lane * 4, w + static_cast<long long>(r0 + warp + 8 * i) * p.J + j0 + lane * 4);
                     }
-                }
-            } else {
-                if (rc == 0)
-                    for (int q = tid; q < TM * EN; q += THREADS) {
-                        const int m = row_s[q / EN], n = q % EN;
-                        const bool there = m >= 0 && n < jn;
-                        copy1(cs + q, there ? p.c + static_cast<long long>(m) * p.J + j0 + n : p.c, there);
-                    }
-                if (!RMAJ)
+                } else {
                     for (int q = tid; q < rn * EN; q += THREADS) {
                         const int r = q / EN, n = q % EN;
                         copy1(ws + r * C::LD + n, n < jn ? w + static_cast<long long>(r0 + r) * p.J + j0 + n : p.w, n < jn);
                     }
+                }
             }
             if constexpr (RMAJ) {
                 // B is read along its ranks and stored rank by rank
@@ -440,67 +438,73 @@ __global__ void __launch_bounds__(THREADS, 2) expand_kernel(const ExpandParams p
         }
         commit_copies();
     };
-    issue(0);
+    issue_w(0);
     if (with) {
         const float scale = p.scale ? __ldg(p.scale + tile.adapter) : 1.f;
         for (int e = tid; e < TM * p.rank; e += THREADS) {
             const int r = e / p.rank, c = e - r * p.rank;
-            const float v = row_s[r] >= 0 ? scale * __ldg(p.t + static_cast<long long>(row_s[r]) * p.rank + c) : 0.f;
-            *reinterpret_cast<float2*>(ts + (c * TM + r) * 2) = make_float2(v, v);
+            ts[c * TM + r] = row_s[r] >= 0 ? scale * __ldg(p.t + static_cast<long long>(row_s[r]) * p.rank + c) : 0.f;
         }
     }
-    float2 acc[8][2];
+    float2 acc[4][4];                                      // [pair of rows][column]
     for (int step = 0; step < steps; step++) {
-        issue(step + 1);
-        wait_copies<1>();
-        __syncthreads();
         const int ct = step / rchunks, rc = step - ct * rchunks;
+        wait_copies<0>();                                  // this step's ranks
+        __syncthreads();
+        if (rc == 0) issue_c(ct);
+        commit_copies();
+        issue_w(step + 1);
         const float* ws = wring + (step & 1) * C::W_FLOATS + lane * 4;
         if (rc == 0) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) acc[i][0] = acc[i][1] = make_float2(0.f, 0.f);
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) acc[i][j] = make_float2(0.f, 0.f);
         }
         if (with) {
             const int rn = min(RC, p.rank - rc * RC);
-            const float* tp = ts + (rc * RC * TM + warp * 8) * 2;
+            const float* tp = ts + rc * RC * TM + warp * 8;
 #pragma unroll 4
             for (int r = 0; r < rn; r++) {
                 const float4 wv = *reinterpret_cast<const float4*>(ws + r * C::LD);
+                const float4 t0 = *reinterpret_cast<const float4*>(tp + r * TM);
+                const float4 t1 = *reinterpret_cast<const float4*>(tp + r * TM + 4);
+                const float2 tv[4] = {make_float2(t0.x, t0.y), make_float2(t0.z, t0.w), make_float2(t1.x, t1.y), make_float2(t1.z, t1.w)};
 #pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    const float4 tv = *reinterpret_cast<const float4*>(tp + (r * TM + i) * 2);
-                    acc[i][0] = __ffma2_rn(make_float2(tv.x, tv.y), make_float2(wv.x, wv.y), acc[i][0]);
-                    acc[i][1] = __ffma2_rn(make_float2(tv.x, tv.y), make_float2(wv.z, wv.w), acc[i][1]);
-                    acc[i + 1][0] = __ffma2_rn(make_float2(tv.z, tv.w), make_float2(wv.x, wv.y), acc[i + 1][0]);
-                    acc[i + 1][1] = __ffma2_rn(make_float2(tv.z, tv.w), make_float2(wv.z, wv.w), acc[i + 1][1]);
+                for (int i = 0; i < 4; i++) {
+                    acc[i][0] = __ffma2_rn(tv[i], make_float2(wv.x, wv.x), acc[i][0]);
+                    acc[i][1] = __ffma2_rn(tv[i], make_float2(wv.y, wv.y), acc[i][1]);
+                    acc[i][2] = __ffma2_rn(tv[i], make_float2(wv.z, wv.z), acc[i][2]);
+                    acc[i][3] = __ffma2_rn(tv[i], make_float2(wv.w, wv.w), acc[i][3]);
                 }
             }
         }
-        if (rc == rchunks - 1) {
-            const int j = (ct0 + ct) * EN + lane * 4, left = p.J - j;
-            const float* cs = cring + (ct & 1) * C::C_FLOATS + lane * 4;
+        if (rc < rchunks - 1) continue;
+        wait_copies<1>();                                  // c (the ranks of the next step may still be under way)
+        const int j = (ct0 + ct) * EN + lane * 4, left = p.J - j;
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int m = row_s[warp * 8 + i];
-                if (m < 0 || left <= 0) continue;
-                float4 v = *reinterpret_cast<const float4*>(cs + (warp * 8 + i) * EN);
-                v.x += acc[i][0].x; v.y += acc[i][0].y; v.z += acc[i][1].x; v.w += acc[i][1].y;
-                if (p.act) {
-                    v.x = act_apply(v.x, p.act); v.y = act_apply(v.y, p.act);
-                    v.z = act_apply(v.z, p.act); v.w = act_apply(v.w, p.act);
-                }
-                float* dst = p.c + static_cast<long long>(m) * p.J + j;
-                if (VEC) {
-                    *reinterpret_cast<float4*>(dst) = v;
-                } else {
-                    dst[0] = v.x;
-                    if (left > 1) dst[1] = v.y;
-                    if (left > 2) dst[2] = v.z;
-                    if (left > 3) dst[3] = v.w;
-                }
+        for (int i = 0; i < 8; i++) {
+            const int m = row_s[warp * 8 + i];
+            if (m < 0 || left <= 0) continue;
+            float4 v = *reinterpret_cast<const float4*>(cs + (warp * 8 + i) * EN + lane * 4);
+            v.x += i & 1 ? acc[i / 2][0].y : acc[i / 2][0].x;
+            v.y += i & 1 ? acc[i / 2][1].y : acc[i / 2][1].x;
+            v.z += i & 1 ? acc[i / 2][2].y : acc[i / 2][2].x;
+            v.w += i & 1 ? acc[i / 2][3].y : acc[i / 2][3].x;
+            if (p.act) {
+                v.x = act_apply(v.x, p.act); v.y = act_apply(v.y, p.act);
+                v.z = act_apply(v.z, p.act); v.w = act_apply(v.w, p.act);
+            }
+            float* dst = p.c + static_cast<long long>(m) * p.J + j;
+            if (VEC) {
+                *reinterpret_cast<float4*>(dst) = v;
+            } else {
+                dst[0] = v.x;
+                if (left > 1) dst[1] = v.y;
+                if (left > 2) dst[2] = v.z;
+                if (left > 3) dst[3] = v.w;
             }
         }
-        __syncthreads();
     }
     wait_copies<0>();
 }
@@ -509,7 +513,7 @@ __global__ void __launch_bounds__(THREADS, 2) expand_kernel(const ExpandParams p
 
 // out = small^T . big over one adapter's rows: a tile of RP ranks x 128 columns.  A thread owns RT (8, or 16) ranks x 4
 // columns, a packed multiply-add serves two ranks; the 32 RP / RT threads that cover the tile once form a row group, and the
-// row groups of the CTA share out the rows of every chunk of 32.  The CTAs of a cluster cut the adapter's rows into
+// row groups of the CTA share out the rows of every chunk of 64.  The CTAs of a cluster cut the adapter's rows into
 // contiguous ranges.  Joins as in shrink_kernel.  Two jobs in one grid: dA (rank, K) from dt and x, dB (N, rank) from t
 // and g.
 struct OuterJob {
@@ -528,7 +532,7 @@ struct OuterParams {
 
 template <int RP>
 struct OuterCfg {
-    static constexpr int MC = 32, CN = 128, STAGES = 3, STAGE_FLOATS = MC * CN + MC * RP;
+    static constexpr int MC = 64, CN = 128, STAGES = 2, STAGE_FLOATS = MC * CN + MC * RP;
     static constexpr int RT = RP < 16 ? RP : 16, GROUP = 32 * (RP / RT), MG = THREADS / GROUP;
     static constexpr int RED_FLOATS = MG * RP * CN;
     static constexpr int SMEM_BYTES = (STAGES * STAGE_FLOATS > RED_FLOATS ? STAGES * STAGE_FLOATS : RED_FLOATS) * 4;
@@ -709,7 +713,7 @@ template <int RP, bool KMAJ>
 cudaError_t launch_shrink_t(cudaStream_t st, const ShrinkParams& p, int tiles, bool vec, int num_sms)
 {
     const int rblocks = (p.rank + RP - 1) / RP;
-    const int S = cluster_size(static_cast<long long>(tiles) * rblocks, p.L, 2 * ShrinkCfg<RP, KMAJ>::KC, num_sms);
+    const int S = cluster_size(static_cast<long long>(tiles) * rblocks, p.L, ShrinkCfg<RP, KMAJ>::KC, num_sms);
     const dim3 grid(static_cast<unsigned int>(tiles) * S, rblocks, 1);
     const int smem = ShrinkCfg<RP, KMAJ>::smem_bytes(p.rank);
     return vec ? launch_cluster(st, shrink_kernel<RP, KMAJ, true>, grid, S, smem, p)
@@ -729,7 +733,7 @@ template <int RP>
 cudaError_t launch_outer_t(cudaStream_t st, const OuterParams& p, int groups, int count, bool vec, int num_sms)
 {
     const int tiles = p.job[0].tiles + p.job[1].tiles, rblocks = (p.rank + RP - 1) / RP;
-    const int S = cluster_size(static_cast<long long>(tiles) * rblocks * groups, p.rows / groups, 2 * OuterCfg<RP>::MC, num_sms);
+    const int S = cluster_size(static_cast<long long>(tiles) * rblocks * groups, p.rows / groups, OuterCfg<RP>::MC, num_sms);
     // (without a grouping the adapters behind the first have no rows: their CTAs store zeros)
     const dim3 grid(static_cast<unsigned int>(tiles) * S, count, rblocks);
     return vec ? launch_cluster(st, outer_kernel<RP, true>, grid, S, OuterCfg<RP>::SMEM_BYTES, p)
@@ -841,8 +845,8 @@ cudaError_t launch_expand(cudaStream_t st, const Groups& g, const Adapters& ad, 
     p.rows = rows; p.J = J; p.rank = ad.rank; p.act = act;
     const bool vec = J % 4 == 0 && aligned16(c) && (up || aligned16(p.w));
     const int tiles = g.perm ? g.max_tiles : (rows + TM - 1) / TM, cols = (J + EN - 1) / EN;
-    // column tiles per CTA: as many as leave four CTAs per SM
-    const long long per = static_cast<long long>(tiles) * cols / (4ll * num_sms);
+    // column tiles per CTA: as many as leave six CTAs per SM
+    const long long per = static_cast<long long>(tiles) * cols / (6ll * num_sms);
     p.tiles_per = static_cast<int>(per < 1 ? 1 : per > 8 ? 8 : per);
     const dim3 grid(tiles, (cols + p.tiles_per - 1) / p.tiles_per, 1);
     if (up) {
