@@ -1309,17 +1309,18 @@ TT_API int tt_lora_fwd(tt_handle_t h, void* stream, const tt_lora_desc* lora, co
             return TT_OK;
         }
     }
-    lora::Groups g;
-    if ((rc = lora_group(h, st, lora, row_adapter, M, ws, g))) return rc;
-    e = lora::launch_shrink(st, g, ad, true, false, x, tt, M, K, h->num_sms);
-    if (e != cudaSuccess) return cuda_fail(h, e, "adapter down-projection launch");
-    h->stats.launches++;
+    // the projection first: the adapters' launches behind it overlap one another
     if (w) {
         GemmCall gc{x, w, y, M, N, K, K, 1, 1, K, HostBatch(), 1, Epilogue{bias, TT_ACT_NONE}};
         gc.ws_off = ws.end;
         if ((rc = run_gemm(h, st, gc))) return rc;
     }
-    e = lora::launch_expand(st, g, ad, true, true, tt, y, M, N, act, h->num_sms);
+    lora::Groups g;
+    if ((rc = lora_group(h, st, lora, row_adapter, M, ws, g))) return rc;
+    e = lora::launch_shrink(st, g, ad, true, false, x, tt, M, K, row_adapter != nullptr, h->num_sms);
+    if (e != cudaSuccess) return cuda_fail(h, e, "adapter down-projection launch");
+    h->stats.launches++;
+    e = lora::launch_expand(st, g, ad, true, true, tt, y, M, N, act, true, true, h->num_sms);
     if (e != cudaSuccess) return cuda_fail(h, e, "adapter up-projection launch");
     h->stats.launches++;
     return TT_OK;
@@ -1350,8 +1351,6 @@ TT_API int tt_lora_bwd(tt_handle_t h, void* stream, const tt_lora_desc* lora, co
         return TT_OK;
     }
     const lora::Adapters ad{lora->a, lora->b, lora->scale, lora->adapters, lora->rank};
-    lora::Groups g;
-    if ((rc = lora_group(h, st, lora, row_adapter, M, ws, g))) return rc;
     // g = dy * act'(y) and the bias gradient
     const float* grad = dy;
     if (act != TT_ACT_NONE || dbias) {
@@ -1373,38 +1372,46 @@ TT_API int tt_lora_bwd(tt_handle_t h, void* stream, const tt_lora_desc* lora, co
         if (gbuf) grad = gbuf;
         ws_used += part_bytes;
     }
-    float* dt = reinterpret_cast<float*>(h->workspace + ws.dt);
-    if (dx || da) {
-        if ((e = lora::launch_shrink(st, g, ad, false, true, grad, dt, M, N, h->num_sms)) != cudaSuccess)
-            return cuda_fail(h, e, "adapter gradient launch");
-        h->stats.launches++;
-    }
-    if (db && !t) {
-        float* tt = reinterpret_cast<float*>(h->workspace + ws.t);
-        if ((e = lora::launch_shrink(st, g, ad, true, false, x, tt, M, K, h->num_sms)) != cudaSuccess)
-            return cuda_fail(h, e, "adapter down-projection launch");
-        h->stats.launches++;
-        t = tt;
-    }
-    if (da || db) {
-        if ((e = lora::launch_outer(st, g, ad, dt, x, da, grad, t, db, M, N, K, h->num_sms)) != cudaSuccess)
-            return cuda_fail(h, e, "adapter weight gradient launch");
-        h->stats.launches++;
-    }
-    if (dx) {
-        if (w) {
-            GemmCall gx{grad, w, dx, M, K, N, N, 1, K, 1, HostBatch(), 1, Epilogue{nullptr, TT_ACT_NONE}};
-            gx.ws_off = ws_used;
-            if ((rc = run_gemm(h, st, gx))) return rc;
-        }
-        if ((e = lora::launch_expand(st, g, ad, false, false, dt, dx, M, K, TT_ACT_NONE, h->num_sms)) != cudaSuccess)
-            return cuda_fail(h, e, "adapter input gradient launch");
-        h->stats.launches++;
+    // the projection's products, then the adapters' launches, which overlap one another
+    if (dx && w) {
+        GemmCall gx{grad, w, dx, M, K, N, N, 1, K, 1, HostBatch(), 1, Epilogue{nullptr, TT_ACT_NONE}};
+        gx.ws_off = ws_used;
+        if ((rc = run_gemm(h, st, gx))) return rc;
     }
     if (dw) {
         GemmCall gw{grad, x, dw, N, K, M, 1, N, K, 1, HostBatch(), 1, Epilogue{nullptr, TT_ACT_NONE}};
         gw.ws_off = ws_used;
         if ((rc = run_gemm(h, st, gw))) return rc;
+    }
+    lora::Groups g;
+    if ((rc = lora_group(h, st, lora, row_adapter, M, ws, g))) return rc;
+    bool early = row_adapter != nullptr;
+    float* dt = reinterpret_cast<float*>(h->workspace + ws.dt);
+    if (dx || da) {
+        if ((e = lora::launch_shrink(st, g, ad, false, true, grad, dt, M, N, early, h->num_sms)) != cudaSuccess)
+            return cuda_fail(h, e, "adapter gradient launch");
+        h->stats.launches++;
+        early = true;
+    }
+    const bool t_is_new = db && !t;
+    if (t_is_new) {
+        float* tt = reinterpret_cast<float*>(h->workspace + ws.t);
+        if ((e = lora::launch_shrink(st, g, ad, true, false, x, tt, M, K, early, h->num_sms)) != cudaSuccess)
+            return cuda_fail(h, e, "adapter down-projection launch");
+        h->stats.launches++;
+        early = true;
+        t = tt;
+    }
+    if (da || db) {
+        if ((e = lora::launch_outer(st, g, ad, dt, x, da, grad, t, db, M, N, K, t_is_new, early, h->num_sms)) != cudaSuccess)
+            return cuda_fail(h, e, "adapter weight gradient launch");
+        h->stats.launches++;
+        early = true;
+    }
+    if (dx) {
+        if ((e = lora::launch_expand(st, g, ad, false, false, dt, dx, M, K, TT_ACT_NONE, early, !(da || db), h->num_sms)) != cudaSuccess)
+            return cuda_fail(h, e, "adapter input gradient launch");
+        h->stats.launches++;
     }
     return TT_OK;
 }

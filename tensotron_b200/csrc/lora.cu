@@ -27,6 +27,20 @@ constexpr int THREADS = 256;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// The launches of a call overlap: each lets the next one begin (let_next_begin) once the launches in front of it are known
+// to be complete, and waits (wait_for_previous) where it first reads what the one in front of it writes, or at its end.  So
+// at any point behind a wait, and at the start of a launch that was let begin, everything but the launch directly in
+// front is complete.
+__device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// At the end of a kernel whose CTAs need not have waited: one of them does, so that this launch is not complete before the
+// one in front of it, and the others leave their SM.
+__device__ __forceinline__ void finish()
+{
+    if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) wait_for_previous();
+}
+
 // ---- grouping of the rows -----------------------------------------------------------------------
 
 // One CTA per group (adapters 0 .. count-1, then the rows without one).  A CTA counts the rows of all lower groups and,
@@ -39,6 +53,7 @@ group_kernel(Groups g, const int* __restrict__ row_adapter, int rows, int count,
     constexpr int WARPS = THREADS / 32;
     __shared__ int below_s[WARPS], own_s[WARPS], carry_s[WARPS];
     __shared__ unsigned int last;
+    let_next_begin();
     const int e = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int per = ((rows + WARPS - 1) / WARPS + 31) & ~31;
     const int r0 = warp * per, r1 = min(rows, r0 + per);
@@ -129,11 +144,11 @@ __device__ __forceinline__ Tile tile_of(const Groups& g, int i, int rows)
 {
     Tile t;
     if (g.perm) {
-        t.valid = i < __ldg(g.n_tiles);
+        t.valid = i < __ldcg(g.n_tiles);
         if (!t.valid) return t;
-        t.adapter = __ldg(g.tile_adapter + i);
-        t.first = __ldg(g.tile_first + i);
-        t.rows = __ldg(g.tile_rows + i);
+        t.adapter = __ldcg(g.tile_adapter + i);
+        t.first = __ldcg(g.tile_first + i);
+        t.rows = __ldcg(g.tile_rows + i);
     } else {
         t.adapter = 0;
         t.first = i * TM;
@@ -147,7 +162,7 @@ __device__ __forceinline__ Tile tile_of(const Groups& g, int i, int rows)
 __device__ __forceinline__ void tile_row_numbers(const Groups& g, const Tile& tile, int* row_s)
 {
     if (threadIdx.x < TM)
-        row_s[threadIdx.x] = static_cast<int>(threadIdx.x) < tile.rows ? (g.perm ? __ldg(g.perm + tile.first + threadIdx.x) : tile.first + static_cast<int>(threadIdx.x)) : -1;
+        row_s[threadIdx.x] = static_cast<int>(threadIdx.x) < tile.rows ? (g.perm ? __ldcg(g.perm + tile.first + threadIdx.x) : tile.first + static_cast<int>(threadIdx.x)) : -1;
 }
 
 // The tiled kernels take their operands through rings of stages filled by asynchronous copies, of 16 bytes where every row
@@ -159,8 +174,8 @@ __device__ __forceinline__ void tile_row_numbers(const Groups& g, const Tile& ti
 
 // ---- shrink ---------------------------------------------------------------------------------------
 
-// A tile of 64 rows x RP ranks.  A thread owns 4 rows x 8 ranks; the 2 RP threads that cover the tile once form a k group,
-// and the 128 / RP k groups of the CTA share out the contraction index of every chunk of 128.  KMAJ: both operands
+// A tile of 64 rows x RP ranks.  A thread owns 4 rows x RT ranks; the threads that cover the tile once form a k group, and
+// the k groups of the CTA share out the contraction index of every chunk of KC.  KMAJ: both operands
 // have the contraction index contiguous, a 128-bit load of each makes two packed multiply-adds per output (sums over even
 // and odd indices, added at the end); otherwise the ranks are contiguous and a packed multiply-add serves two of them.  The
 // CTAs of a cluster cut the contraction into contiguous ranges; k groups are added through shared memory, the cluster's
@@ -176,8 +191,11 @@ struct ShrinkParams {
 
 template <int RP, bool KMAJ>
 struct ShrinkCfg {
-    static constexpr int KC = 128, LD = KC + 4, STAGES = 2, X_FLOATS = TM * LD;
-    static constexpr int RED_FLOATS = 128 / RP * TM * RP;
+    static constexpr int RT = KMAJ ? 4 : 8;                  // ranks per thread
+    static constexpr int KC = KMAJ ? 64 : 128, LD = KC + 4, STAGES = KMAJ ? 3 : 2, X_FLOATS = TM * LD;
+    static constexpr int GROUP = 16 * RP / RT, KG = THREADS / GROUP;
+    static constexpr int MIN_CTAS = KMAJ ? 3 : 2;
+    static constexpr int RED_FLOATS = KG * TM * RP;
     // row pitch of the adapter's part of a stage, and its floats (ranks behind the last one are read past a row's end)
     __host__ __device__ static int pitch(int rank) { return KMAJ ? LD : (rank + 3) & ~3; }
     __host__ __device__ static int w_floats(int rank) { return KMAJ ? RP * LD : KC * pitch(rank) + RP; }
@@ -189,16 +207,18 @@ struct ShrinkCfg {
 };
 
 template <int RP, bool KMAJ, bool VEC>
-__global__ void __launch_bounds__(THREADS, 2) shrink_kernel(const ShrinkParams p)
+__global__ void __launch_bounds__(THREADS, (ShrinkCfg<RP, KMAJ>::MIN_CTAS)) shrink_kernel(const ShrinkParams p)
 {
     using C = ShrinkCfg<RP, KMAJ>;
-    constexpr int KC = C::KC, LD = C::LD, STAGES = C::STAGES, GROUP = 2 * RP, KG = THREADS / GROUP, QPG = KC / 4 / KG;
+    constexpr int KC = C::KC, LD = C::LD, STAGES = C::STAGES, RT = C::RT, GROUP = C::GROUP, KG = C::KG, QPG = KC / 4 / KG;
     extern __shared__ __align__(16) float smem[];
     __shared__ int row_s[TM];
     cg::cluster_group cluster = cg::this_cluster();
     const int S = static_cast<int>(cluster.num_blocks()), split = static_cast<int>(cluster.block_rank());
     const int tid = threadIdx.x;
     const int rb = blockIdx.y * RP;                                  // first rank of this block of ranks
+    wait_for_previous();
+    let_next_begin();
     const Tile tile = tile_of(p.g, blockIdx.x / S, p.rows);
     if (!tile.valid) return;                                         // (the whole cluster)
     tile_row_numbers(p.g, tile, row_s);
@@ -263,11 +283,11 @@ __global__ void __launch_bounds__(THREADS, 2) shrink_kernel(const ShrinkParams p
     };
 
     const int kg = tid / GROUP, t = tid % GROUP, rg = t % 16, cgp = t / 16;
-    float2 acc[4][8];                          // KMAJ: (even, odd) sums per rank; else [4][0..3]: rank pairs
+    float2 acc[4][4];                          // KMAJ: (even, odd) sums of four ranks; else four rank pairs
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int j = 0; j < 8; j++) acc[i][j] = make_float2(0.f, 0.f);
+        for (int j = 0; j < 4; j++) acc[i][j] = make_float2(0.f, 0.f);
     for (int s = 0; s < STAGES - 1; s++) issue(s);
     for (int done = 0; done < chunks; done++) {
         wait_copies<STAGES - 2>();
@@ -285,8 +305,8 @@ __global__ void __launch_bounds__(THREADS, 2) shrink_kernel(const ShrinkParams p
             for (int i = 0; i < 4; i++) xv[i] = *reinterpret_cast<const float4*>(xs + (rg + 16 * i) * LD + k);
             if constexpr (KMAJ) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const float4 wv = *reinterpret_cast<const float4*>(ws + (cgp + RP / 8 * j) * LD + k);
+                for (int j = 0; j < 4; j++) {
+                    const float4 wv = *reinterpret_cast<const float4*>(ws + (cgp + RP / 4 * j) * LD + k);
 #pragma unroll
                     for (int i = 0; i < 4; i++) acc[i][j] = __ffma2_rn(make_float2(xv[i].x, xv[i].y), make_float2(wv.x, wv.y), acc[i][j]);
 #pragma unroll
@@ -315,9 +335,9 @@ __global__ void __launch_bounds__(THREADS, 2) shrink_kernel(const ShrinkParams p
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int j = 0; j < 8; j++)
-            smem[(kg * TM + rg + 16 * i) * RP + (KMAJ ? cgp + RP / 8 * j : cgp * 8 + j)] =
-                KMAJ ? acc[i][j].x + acc[i][j].y : (j & 1 ? acc[i][j / 2].y : acc[i][j / 2].x);
+        for (int j = 0; j < RT; j++)
+            smem[(kg * TM + rg + 16 * i) * RP + (KMAJ ? cgp + RP / 4 * j : cgp * 8 + j)] =
+                KMAJ ? acc[i][j % 4].x + acc[i][j % 4].y : (j & 1 ? acc[i][j / 2].y : acc[i][j / 2].x);
     __syncthreads();
     for (int e = tid; e < TM * RP && KG > 1; e += THREADS) {
         float s = smem[e];
@@ -327,9 +347,8 @@ __global__ void __launch_bounds__(THREADS, 2) shrink_kernel(const ShrinkParams p
     }
     const float scale = p.scale && tile.adapter >= 0 ? __ldg(p.scale + tile.adapter) : 1.f;
     if (S > 1) cluster.sync(); else __syncthreads();
-    const int rows_per = TM / S;
-    for (int e = tid; e < rows_per * RP; e += THREADS) {
-        const int r = split * rows_per + e / RP, c = e % RP;
+    for (int e = split * THREADS + tid; e < TM * RP; e += S * THREADS) {
+        const int r = e / RP, c = e % RP;
         if (row_s[r] < 0 || rb + c >= p.rank) continue;
         float s = S > 1 ? *cluster.map_shared_rank(smem + r * RP + c, 0) : smem[r * RP + c];
         for (int q = 1; q < S; q++) s += *cluster.map_shared_rank(smem + r * RP + c, q);
@@ -351,6 +370,7 @@ struct ExpandParams {
     const float* scale;   // (count) or null
     float* c;             // (rows, J)
     int rows, J, rank, act, tiles_per;
+    int wait_first;       // the launch in front writes t, or c
 };
 
 constexpr int EN = 128;
@@ -368,7 +388,11 @@ __global__ void __launch_bounds__(THREADS, 3) expand_kernel(const ExpandParams p
     extern __shared__ __align__(16) float smem[];
     __shared__ int row_s[TM];
     const Tile tile = tile_of(p.g, blockIdx.x, p.rows);
-    if (!tile.valid || (tile.adapter < 0 && p.act == 0)) return;
+    if (p.wait_first) wait_for_previous();
+    if (!tile.valid || (tile.adapter < 0 && p.act == 0)) {
+        finish();
+        return;
+    }
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const bool with = tile.adapter >= 0;
     const int rchunks = with ? (p.rank + RC - 1) / RC : 1;
@@ -443,7 +467,7 @@ __global__ void __launch_bounds__(THREADS, 3) expand_kernel(const ExpandParams p
         const float scale = p.scale ? __ldg(p.scale + tile.adapter) : 1.f;
         for (int e = tid; e < TM * p.rank; e += THREADS) {
             const int r = e / p.rank, c = e - r * p.rank;
-            ts[c * TM + r] = row_s[r] >= 0 ? scale * __ldg(p.t + static_cast<long long>(row_s[r]) * p.rank + c) : 0.f;
+            ts[c * TM + r] = row_s[r] >= 0 ? scale * __ldcg(p.t + static_cast<long long>(row_s[r]) * p.rank + c) : 0.f;
         }
     }
     float2 acc[4][4];                                      // [pair of rows][column]
@@ -507,6 +531,7 @@ __global__ void __launch_bounds__(THREADS, 3) expand_kernel(const ExpandParams p
         }
     }
     wait_copies<0>();
+    finish();
 }
 
 // ---- outer ----------------------------------------------------------------------------------------
@@ -522,6 +547,7 @@ struct OuterJob {
     float* out;           // (count, rank, C), or (count, C, rank) when col_major
     const float* scale;   // (count) or null
     int C, col_major, tiles;
+    int wait_first;       // the launch in front writes `small` (or nobody else waits for it)
 };
 
 struct OuterParams {
@@ -550,6 +576,8 @@ __global__ void __launch_bounds__(THREADS, 2) outer_kernel(const OuterParams p)
     int ct = blockIdx.x / S;
     const OuterJob& job = p.job[ct < p.job[0].tiles ? 0 : 1];
     if (ct >= p.job[0].tiles) ct -= p.job[0].tiles;
+    if (job.wait_first) wait_for_previous();
+    let_next_begin();
     const int c0 = ct * CN, cn = min(CN, job.C - c0), rn = min(RP, p.rank - rb);
     int first = 0, n = p.rows;
     if (p.g.perm) {
@@ -661,9 +689,7 @@ __global__ void __launch_bounds__(THREADS, 2) outer_kernel(const OuterParams p)
     const float scale = job.scale ? __ldg(job.scale + e) : 1.f;
     float* out = job.out + static_cast<long long>(e) * p.rank * job.C;
     if (S > 1) cluster.sync(); else __syncthreads();
-    const int per = RP * CN / S;
-    for (int q = tid; q < per; q += THREADS) {
-        const int k = split * per + q;
+    for (int k = split * THREADS + tid; k < RP * CN; k += S * THREADS) {
         // neighbouring threads write neighbouring addresses in either layout
         const int r = job.col_major ? k % RP : k / CN, c = job.col_major ? k / RP : k % CN;
         if (r >= rn || c >= cn) continue;
@@ -672,23 +698,27 @@ __global__ void __launch_bounds__(THREADS, 2) outer_kernel(const OuterParams p)
         out[job.col_major ? static_cast<long long>(c0 + c) * p.rank + rb + r : static_cast<long long>(rb + r) * job.C + c0 + c] = scale * s;
     }
     if (S > 1) cluster.sync();
+    finish();
 }
 
+// `early`: the launch in front of this one is one of these kernels (it lets this one begin once all its CTAs run).
 template <typename P>
-cudaError_t launch_cluster(cudaStream_t st, void (*kernel)(P), dim3 grid, int cluster, int smem, const P& p)
+cudaError_t launch_cluster(cudaStream_t st, void (*kernel)(P), dim3 grid, int cluster, int smem, bool early, const P& p)
 {
     cudaLaunchConfig_t cfg = {};
     cfg.dynamicSmemBytes = smem;
     cfg.gridDim = grid;
     cfg.blockDim = dim3(THREADS, 1, 1);
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = static_cast<unsigned int>(cluster);
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = early ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
@@ -701,43 +731,43 @@ int tile_bound(int rows, int adapters)
     return rows / TM + groups;
 }
 
-// Clusters of a launch: doubled while the CTAs still fit the SMs once, two on each, and `longest` leaves enough work per CTA.
-int cluster_size(long long ctas, int longest, int least, int num_sms)
+// CTAs of a cluster: as many as let all CTAs be resident at once, `per_sm` on each SM, with at least `least` of the
+// `longest` contraction for each.
+int cluster_size(long long ctas, int longest, int least, int per_sm, int num_sms)
 {
     int S = 1;
-    while (S < 8 && ctas * S * 2 <= 2ll * num_sms && longest / (2 * S) >= least) S *= 2;
+    while (S < 8 && ctas * (S + 1) <= static_cast<long long>(per_sm) * num_sms && longest / (S + 1) >= least) S++;
     return S;
 }
 
 template <int RP, bool KMAJ>
-cudaError_t launch_shrink_t(cudaStream_t st, const ShrinkParams& p, int tiles, bool vec, int num_sms)
+cudaError_t launch_shrink_t(cudaStream_t st, const ShrinkParams& p, int tiles, bool vec, bool early, int num_sms)
 {
     const int rblocks = (p.rank + RP - 1) / RP;
-    const int S = cluster_size(static_cast<long long>(tiles) * rblocks, p.L, ShrinkCfg<RP, KMAJ>::KC, num_sms);
+    const int S = cluster_size(static_cast<long long>(tiles) * rblocks, p.L, 128, ShrinkCfg<RP, KMAJ>::MIN_CTAS, num_sms);
     const dim3 grid(static_cast<unsigned int>(tiles) * S, rblocks, 1);
     const int smem = ShrinkCfg<RP, KMAJ>::smem_bytes(p.rank);
-    return vec ? launch_cluster(st, shrink_kernel<RP, KMAJ, true>, grid, S, smem, p)
-                : launch_cluster(st, shrink_kernel<RP, KMAJ, false>, grid, S, smem, p);
+    return vec ? launch_cluster(st, shrink_kernel<RP, KMAJ, true>, grid, S, smem, early, p)
+               : launch_cluster(st, shrink_kernel<RP, KMAJ, false>, grid, S, smem, early, p);
 }
 
 template <int RC, bool RMAJ>
-cudaError_t launch_expand_t(cudaStream_t st, const ExpandParams& p, dim3 grid, bool vec)
+cudaError_t launch_expand_t(cudaStream_t st, const ExpandParams& p, dim3 grid, bool vec, bool early)
 {
     const int smem = ExpandCfg<RC>::smem_bytes(p.rank);
-    if (vec) expand_kernel<RC, RMAJ, true><<<grid, THREADS, smem, st>>>(p);
-    else      expand_kernel<RC, RMAJ, false><<<grid, THREADS, smem, st>>>(p);
-    return cudaGetLastError();
+    return vec ? launch_cluster(st, expand_kernel<RC, RMAJ, true>, grid, 1, smem, early, p)
+               : launch_cluster(st, expand_kernel<RC, RMAJ, false>, grid, 1, smem, early, p);
 }
 
 template <int RP>
-cudaError_t launch_outer_t(cudaStream_t st, const OuterParams& p, int groups, int count, bool vec, int num_sms)
+cudaError_t launch_outer_t(cudaStream_t st, const OuterParams& p, int groups, int count, bool vec, bool early, int num_sms)
 {
     const int tiles = p.job[0].tiles + p.job[1].tiles, rblocks = (p.rank + RP - 1) / RP;
-    const int S = cluster_size(static_cast<long long>(tiles) * rblocks * groups, p.rows / groups, OuterCfg<RP>::MC, num_sms);
+    const int S = cluster_size(static_cast<long long>(tiles) * rblocks * groups, p.rows / groups, OuterCfg<RP>::MC, 2, num_sms);
     // (without a grouping the adapters behind the first have no rows: their CTAs store zeros)
     const dim3 grid(static_cast<unsigned int>(tiles) * S, count, rblocks);
-    return vec ? launch_cluster(st, outer_kernel<RP, true>, grid, S, OuterCfg<RP>::SMEM_BYTES, p)
-                : launch_cluster(st, outer_kernel<RP, false>, grid, S, OuterCfg<RP>::SMEM_BYTES, p);
+    return vec ? launch_cluster(st, outer_kernel<RP, true>, grid, S, OuterCfg<RP>::SMEM_BYTES, early, p)
+               : launch_cluster(st, outer_kernel<RP, false>, grid, S, OuterCfg<RP>::SMEM_BYTES, early, p);
 }
 
 template <typename K>
@@ -810,7 +840,7 @@ cudaError_t init_tiled()
 }
 
 cudaError_t launch_shrink(cudaStream_t st, const Groups& g, const Adapters& ad, bool down, bool scaled, const float* x,
-                          float* out, int rows, int L, int num_sms)
+                          float* out, int rows, int L, bool early, int num_sms)
 {
     ShrinkParams p;
     p.g = g;
@@ -822,19 +852,19 @@ cudaError_t launch_shrink(cudaStream_t st, const Groups& g, const Adapters& ad, 
     const bool vec = L % 4 == 0 && aligned16(x) && aligned16(p.w) && (down || ad.rank % 4 == 0);
     const int tiles = g.perm ? g.max_tiles : (rows + TM - 1) / TM;
     if (down) {
-        if (ad.rank <= 8)  return launch_shrink_t<8, true>(st, p, tiles, vec, num_sms);
-        if (ad.rank <= 16) return launch_shrink_t<16, true>(st, p, tiles, vec, num_sms);
-        if (ad.rank <= 32) return launch_shrink_t<32, true>(st, p, tiles, vec, num_sms);
-        return launch_shrink_t<64, true>(st, p, tiles, vec, num_sms);
+        if (ad.rank <= 8)  return launch_shrink_t<8, true>(st, p, tiles, vec, early, num_sms);
+        if (ad.rank <= 16) return launch_shrink_t<16, true>(st, p, tiles, vec, early, num_sms);
+        if (ad.rank <= 32) return launch_shrink_t<32, true>(st, p, tiles, vec, early, num_sms);
+        return launch_shrink_t<64, true>(st, p, tiles, vec, early, num_sms);
     }
-    if (ad.rank <= 8)  return launch_shrink_t<8, false>(st, p, tiles, vec, num_sms);
-    if (ad.rank <= 16) return launch_shrink_t<16, false>(st, p, tiles, vec, num_sms);
-    if (ad.rank <= 32) return launch_shrink_t<32, false>(st, p, tiles, vec, num_sms);
-    return launch_shrink_t<64, false>(st, p, tiles, vec, num_sms);
+    if (ad.rank <= 8)  return launch_shrink_t<8, false>(st, p, tiles, vec, early, num_sms);
+    if (ad.rank <= 16) return launch_shrink_t<16, false>(st, p, tiles, vec, early, num_sms);
+    if (ad.rank <= 32) return launch_shrink_t<32, false>(st, p, tiles, vec, early, num_sms);
+    return launch_shrink_t<64, false>(st, p, tiles, vec, early, num_sms);
 }
 
 cudaError_t launch_expand(cudaStream_t st, const Groups& g, const Adapters& ad, bool up, bool scaled, const float* t,
-                          float* c, int rows, int J, int act, int num_sms)
+                          float* c, int rows, int J, int act, bool early, bool wait_first, int num_sms)
 {
     ExpandParams p;
     p.g = g;
@@ -842,7 +872,7 @@ cudaError_t launch_expand(cudaStream_t st, const Groups& g, const Adapters& ad, 
     p.w = up ? ad.b : ad.a;
     p.scale = scaled ? ad.scale : nullptr;
     p.c = c;
-    p.rows = rows; p.J = J; p.rank = ad.rank; p.act = act;
+    p.rows = rows; p.J = J; p.rank = ad.rank; p.act = act; p.wait_first = wait_first;
     const bool vec = J % 4 == 0 && aligned16(c) && (up || aligned16(p.w));
     const int tiles = g.perm ? g.max_tiles : (rows + TM - 1) / TM, cols = (J + EN - 1) / EN;
     // column tiles per CTA: as many as leave six CTAs per SM
@@ -850,17 +880,18 @@ cudaError_t launch_expand(cudaStream_t st, const Groups& g, const Adapters& ad, 
     p.tiles_per = static_cast<int>(per < 1 ? 1 : per > 8 ? 8 : per);
     const dim3 grid(tiles, (cols + p.tiles_per - 1) / p.tiles_per, 1);
     if (up) {
-        if (ad.rank <= 8)  return launch_expand_t<8, true>(st, p, grid, vec);
-        if (ad.rank <= 16) return launch_expand_t<16, true>(st, p, grid, vec);
-        return launch_expand_t<32, true>(st, p, grid, vec);
+        if (ad.rank <= 8)  return launch_expand_t<8, true>(st, p, grid, vec, early);
+        if (ad.rank <= 16) return launch_expand_t<16, true>(st, p, grid, vec, early);
+        return launch_expand_t<32, true>(st, p, grid, vec, early);
     }
-    if (ad.rank <= 8)  return launch_expand_t<8, false>(st, p, grid, vec);
-    if (ad.rank <= 16) return launch_expand_t<16, false>(st, p, grid, vec);
-    return launch_expand_t<32, false>(st, p, grid, vec);
+    if (ad.rank <= 8)  return launch_expand_t<8, false>(st, p, grid, vec, early);
+    if (ad.rank <= 16) return launch_expand_t<16, false>(st, p, grid, vec, early);
+    return launch_expand_t<32, false>(st, p, grid, vec, early);
 }
 
 cudaError_t launch_outer(cudaStream_t st, const Groups& g, const Adapters& ad, const float* dt, const float* x, float* da,
-                         const float* grad, const float* t, float* db, int rows, int N, int K, int num_sms)
+                         const float* grad, const float* t, float* db, int rows, int N, int K, bool t_is_new,
+                         bool early, int num_sms)
 {
     OuterParams p;
     p.g = g;
@@ -870,20 +901,20 @@ cudaError_t launch_outer(cudaStream_t st, const Groups& g, const Adapters& ad, c
     p.job[0].tiles = p.job[1].tiles = 0;
     bool vec = ad.rank % 4 == 0;
     if (da) {
-        p.job[jobs++] = OuterJob{dt, x, da, nullptr, K, 0, (K + 127) / 128};
+        p.job[jobs++] = OuterJob{dt, x, da, nullptr, K, 0, (K + 127) / 128, t_is_new ? 0 : 1};
         vec = vec && K % 4 == 0 && aligned16(x) && aligned16(dt);
     }
     if (db) {
-        p.job[jobs++] = OuterJob{t, grad, db, ad.scale, N, 1, (N + 127) / 128};
+        p.job[jobs++] = OuterJob{t, grad, db, ad.scale, N, 1, (N + 127) / 128, t_is_new || !da ? 1 : 0};
         vec = vec && N % 4 == 0 && aligned16(grad) && aligned16(t);
     }
     if (jobs == 0) return cudaSuccess;
     if (jobs == 1) { p.job[1] = p.job[0]; p.job[1].tiles = 0; }
     const int groups = g.perm ? ad.count : 1;
-    if (ad.rank <= 8)  return launch_outer_t<8>(st, p, groups, ad.count, vec, num_sms);
-    if (ad.rank <= 16) return launch_outer_t<16>(st, p, groups, ad.count, vec, num_sms);
-    if (ad.rank <= 32) return launch_outer_t<32>(st, p, groups, ad.count, vec, num_sms);
-    return launch_outer_t<64>(st, p, groups, ad.count, vec, num_sms);
+    if (ad.rank <= 8)  return launch_outer_t<8>(st, p, groups, ad.count, vec, early, num_sms);
+    if (ad.rank <= 16) return launch_outer_t<16>(st, p, groups, ad.count, vec, early, num_sms);
+    if (ad.rank <= 32) return launch_outer_t<32>(st, p, groups, ad.count, vec, early, num_sms);
+    return launch_outer_t<64>(st, p, groups, ad.count, vec, early, num_sms);
 }
 
 }  // namespace lora

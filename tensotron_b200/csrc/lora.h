@@ -39,20 +39,24 @@ Groups groups_layout(void* mem, int rows, int adapters);
 cudaError_t launch_group(cudaStream_t st, const Groups& g, const int* row_adapter, int rows, int adapters,
                          unsigned int* ticket, unsigned int* status);
 
+// `early`: the launch directly in front, on the same stream, is one of this file's and of the same call; the two then
+// overlap.  `wait_first`: it is the one that writes t or c.  `t_is_new`: it is the one that writes t (else dt, if any).
+
 // out[m, r] = (scaled ? scale[e_m] : 1) * sum_l x[m, l] * W_e[r, l], zeros for rows without an adapter.  W = ad.a
 // (down = true, L = K) or the transposed view of ad.b (down = false, L = N).
 cudaError_t launch_shrink(cudaStream_t st, const Groups& g, const Adapters& ad, bool down, bool scaled, const float* x,
-                          float* out, int rows, int L, int num_sms);
+                          float* out, int rows, int L, bool early, int num_sms);
 
 // c[m, j] = act(c[m, j] + (scaled ? scale[e_m] : 1) * sum_r t[m, r] * W_e[j, r]), W = ad.b (up = true, J = N) or the
 // transposed view of ad.a (up = false, J = K).
 cudaError_t launch_expand(cudaStream_t st, const Groups& g, const Adapters& ad, bool up, bool scaled, const float* t,
-                          float* c, int rows, int J, int act, int num_sms);
+                          float* c, int rows, int J, int act, bool early, bool wait_first, int num_sms);
 
 // da[e] = sum over e's rows of dt[m]^T x[m]   (rank, K)      skipped when da is null
 // db[e] = scale[e] * sum over e's rows of g[m]^T t[m]  (N, rank)      skipped when db is null
 cudaError_t launch_outer(cudaStream_t st, const Groups& g, const Adapters& ad, const float* dt, const float* x, float* da,
-                         const float* grad, const float* t, float* db, int rows, int N, int K, int num_sms);
+                         const float* grad, const float* t, float* db, int rows, int N, int K, bool t_is_new,
+                         bool early, int num_sms);
 
 // The forward pass of at most MAX_FEW_ROWS rows in two launches (lora_rows.cu), without a grouping; *taken = false, and
 // nothing enqueued, when the call is outside what they hold.  t: (M, rank), always written.
