@@ -252,7 +252,7 @@ class TensorRuntime:
         import torch
         # (the raw handle where torch gives it without building a Stream object: 0.1 us instead of 1.5 us per call)
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-        self._current_stream = raw or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+        self._current_stream = raw or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
     # -- lifetime ---------------------------------------------------------------
     def Dispose(self):
@@ -285,7 +285,7 @@ class TensorRuntime:
         """CUstream for the call: explicit, else torch's current stream on this device."""
         if stream is not None:
             return ctypes.c_void_p(stream if isinstance(stream, int) else stream.cuda_stream)
-        return self._current_stream(self.device)
+        return ctypes.c_void_p(self._current_stream(self.device))
 
     # -- math mode (src/Tensotron/TensorRuntime.cs:158-159, :332-338) --------------
     @property
