@@ -45,8 +45,8 @@ namespace {
 
 constexpr size_t DEFAULT_WORKSPACE = 256ull << 20;
 // Device words owned by the handle: word 0 = status of the bounded waits; from word 64 on, one
-// stream-K flag per CTA (zero between launches); behind them the tickets of kernels whose last CTA finishes the job.
-constexpr int STREAMK_FLAGS_WORD = 64, GROUP_TICKET_WORD = 960, LIST_TICKET_WORD = 992, HANDLE_WORDS = 1024;
+// stream-K flag per CTA (zero between launches); behind them the ticket of kernels whose last CTA finishes the job.
+constexpr int STREAMK_FLAGS_WORD = 64, LIST_TICKET_WORD = 992, HANDLE_WORDS = 1024;
 constexpr long long TMA_MIN_FLOP_ELEMS = 1ll << 21;  // M*N*K below this -> any-stride kernel
 constexpr long long SMALL_3XTF32_MAX_ELEMS = 1ll << 28;  // M x N x K up to which 3xTF32 runs on the strict-FP32 kernels
 constexpr long long LINEAR_SMALL_MAX_ELEMS = 1ll << 21;  // M x N x K up to which a Linear backward is ONE launch (linear_small.cuh)
@@ -1256,7 +1256,7 @@ int lora_check(tt_handle_t h, const tt_lora_desc* lora, int M, int N, int K, int
     if (lora->adapters > TT_LORA_MAX_ADAPTERS || lora->rank > TT_LORA_MAX_RANK)
         return fail(h, TT_ERR_UNSUPPORTED, "more adapters or a higher rank than the kernels take");
     if (!lora->a || !lora->b) return fail(h, TT_ERR_INVALID_ARG, "null device pointer");
-    if (static_cast<long long>(M) * lora->rank > 0x7fffffffll || static_cast<long long>(M) * N > 0x7fffffffll ||
+    if (M > (1 << 30) || static_cast<long long>(M) * lora->rank > 0x7fffffffll || static_cast<long long>(M) * N > 0x7fffffffll ||
         static_cast<long long>(M) * K > 0x7fffffffll || (N + 127) / 128 > 65535 || (K + 127) / 128 > 65535)
         return fail(h, TT_ERR_UNSUPPORTED, "more elements than int32 offsets reach");   // like every buffer of the reference
     return TT_OK;
@@ -1269,7 +1269,7 @@ int lora_group(tt_handle_t h, cudaStream_t st, const tt_lora_desc* lora, const i
     g = lora::Groups();
     if (!row_adapter) return TT_OK;
     g = lora::groups_layout(h->workspace + ws.groups, M, lora->adapters);
-    const cudaError_t e = lora::launch_group(st, g, row_adapter, M, lora->adapters, h->status + GROUP_TICKET_WORD, h->status);
+    const cudaError_t e = lora::launch_group(st, g, row_adapter, M, lora->adapters, h->status);
     if (e != cudaSuccess) return cuda_fail(h, e, "row grouping launch");
     h->stats.launches++;
     return TT_OK;

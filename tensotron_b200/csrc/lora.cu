@@ -23,7 +23,7 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 256, GROUP_THREADS = 1024;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -45,20 +45,19 @@ __device__ __forceinline__ void finish()
 
 // One CTA per group (adapters 0 .. count-1, then the rows without one).  A CTA counts the rows of all lower groups and,
 // warp by warp over contiguous row ranges, its own; the range counts give every warp its place, and a second walk
-// writes the row indices.  No atomics on the data: ascending row order within a group, whatever the timing.  The
-// last CTA to finish lists the tiles.
-__global__ void __launch_bounds__(THREADS)
-group_kernel(Groups g, const int* __restrict__ row_adapter, int rows, int count, unsigned int* ticket, unsigned int* status)
+// writes the row indices.  No atomics: ascending row order within a group, whatever the timing.
+__global__ void __launch_bounds__(GROUP_THREADS)
+group_kernel(Groups g, const int* __restrict__ row_adapter, int rows, int count, unsigned int* status)
 {
-    constexpr int WARPS = THREADS / 32;
-    __shared__ int below_s[WARPS], own_s[WARPS], carry_s[WARPS];
-    __shared__ unsigned int last;
+    constexpr int WARPS = GROUP_THREADS / 32, AHEAD = 4;
+    __shared__ int below_s[WARPS], own_s[WARPS];
     let_next_begin();
     const int e = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int per = ((rows + WARPS - 1) / WARPS + 31) & ~31;
     const int r0 = warp * per, r1 = min(rows, r0 + per);
     int below = 0, own = 0;
     bool bad = false;
+#pragma unroll 8
     for (int r = r0 + lane; r < r1; r += 32) {
         int k = __ldg(row_adapter + r);
         if (k < 0 || k >= count) {
@@ -81,81 +80,82 @@ group_kernel(Groups g, const int* __restrict__ row_adapter, int rows, int count,
     }
     int at = base + mine;
     if (total > 0) {
-        for (int r = r0; r < r1; r += 32) {
-            int k = r + lane < r1 ? __ldg(row_adapter + r + lane) : count + 1;
-            if (r + lane < r1 && (k < 0 || k >= count)) k = count;
-            const unsigned int hit = __ballot_sync(0xffffffffu, k == e);
-            if (k == e) g.perm[at + __popc(hit & ((1u << lane) - 1u))] = r + lane;
-            at += __popc(hit);
+        for (int r = r0; r < r1; r += 32 * AHEAD) {
+            int k[AHEAD];
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) {
+                const int at_row = r + 32 * i + lane;
+                k[i] = at_row < r1 ? __ldg(row_adapter + at_row) : e + 1;                 // (not this group's)
+                if (at_row < r1 && (k[i] < 0 || k[i] >= count)) k[i] = count;
+            }
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) {
+                const unsigned int hit = __ballot_sync(0xffffffffu, k[i] == e);
+                if (k[i] == e) g.perm[at + __popc(hit & ((1u << lane) - 1u))] = r + 32 * i + lane;
+                at += __popc(hit);
+            }
         }
     }
     if (threadIdx.x == 0) {
         g.offset[e] = base;
         if (e == count) g.offset[count + 1] = rows;
-        __threadfence();
-        last = atomicAdd(ticket, 1u) == gridDim.x - 1 ? 1u : 0u;
     }
-    __syncthreads();
-    if (!last) return;
-    __threadfence();
-    // tile list: an exclusive scan of ceil(rows / TM) over the groups, THREADS groups at a time
-    int first_tile = 0;
-    for (int g0 = 0; g0 <= count; g0 += THREADS) {
+}
+
+struct Tile {
+    int adapter, first, rows;     // adapter -1: the rows without one
+    bool valid;
+};
+
+// All threads of the CTA: tile `i` of the call.  The tiles follow the groups, ceil(rows / TM) for each, so every CTA finds its
+// own by a scan over the groups' sizes (a list made by the grouping would cost it a second round through memory).
+__device__ __forceinline__ Tile tile_of(const Groups& g, int i, int rows)
+{
+    Tile t;
+    if (!g.perm) {
+        t.adapter = 0;
+        t.first = i * TM;
+        t.rows = min(TM, rows - t.first);
+        t.valid = t.rows > 0;
+        return t;
+    }
+    __shared__ int carry_s[THREADS / 32];
+    __shared__ Tile found;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) found.valid = false;
+    int before = 0;
+    for (int g0 = 0; g0 <= g.count && before <= i; g0 += THREADS) {
         const int k = g0 + threadIdx.x;
         int lo = 0, n = 0;
-        if (k <= count) {
+        if (k <= g.count) {
             lo = __ldcg(g.offset + k);
             n = __ldcg(g.offset + k + 1) - lo;
         }
         const int tiles = (n + TM - 1) / TM;
         int inc = tiles;
+#pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += v;
         }
-        __syncthreads();
         if (lane == 31) carry_s[warp] = inc;
         __syncthreads();
-        int before = first_tile, all = 0;
-        for (int w = 0; w < WARPS; w++) {
-            if (w < warp) before += carry_s[w];
+        int first = before + inc - tiles, all = 0;
+#pragma unroll
+        for (int w = 0; w < THREADS / 32; w++) {
+            if (w < warp) first += carry_s[w];
             all += carry_s[w];
         }
-        int tile = before + inc - tiles;
-        for (int i = 0; i < tiles; i++, tile++) {
-            g.tile_adapter[tile] = k < count ? k : -1;
-            g.tile_first[tile] = lo + i * TM;
-            g.tile_rows[tile] = min(TM, n - i * TM);
+        if (i >= first && i < first + tiles) {
+            found.adapter = k < g.count ? k : -1;
+            found.first = lo + (i - first) * TM;
+            found.rows = min(TM, n - (i - first) * TM);
+            found.valid = true;
         }
-        first_tile += all;
+        before += all;
+        __syncthreads();
     }
-    if (threadIdx.x == 0) {
-        *g.n_tiles = first_tile;
-        *ticket = 0u;
-    }
-}
-
-struct Tile {
-    int adapter, first, rows;
-    bool valid;
-};
-
-__device__ __forceinline__ Tile tile_of(const Groups& g, int i, int rows)
-{
-    Tile t;
-    if (g.perm) {
-        t.valid = i < __ldcg(g.n_tiles);
-        if (!t.valid) return t;
-        t.adapter = __ldcg(g.tile_adapter + i);
-        t.first = __ldcg(g.tile_first + i);
-        t.rows = __ldcg(g.tile_rows + i);
-    } else {
-        t.adapter = 0;
-        t.first = i * TM;
-        t.rows = min(TM, rows - t.first);
-        t.valid = t.rows > 0;
-    }
-    return t;
+    return found;
 }
 
 // Rows of a tile as their numbers in the call, -1 behind the last one.
@@ -169,17 +169,20 @@ __device__ __forceinline__ void tile_row_numbers(const Groups& g, const Tile& ti
 // starts on such a boundary and is a multiple of 16 bytes long (VEC), else of 4.  Every thread copies the same places of
 // every stage, so that a copy costs an addition and the instruction itself.  (Bulk copies, one per row of a stage, were
 // tried: about 45 cycles each per SM whatever their length, 8192 x 4096 rows in 104 us against 55.)  Rows behind the last one
-// of a tile repeat its first (their outputs are not stored); what lies behind the last index of a contraction is 0 or is
+// of a tile repeat its first (their outputs are not stored); the rings start on 128-byte boundaries (16 bytes beside one, the
+// copies of a 512-byte row took an extra pass each: expand_kernel 62 us against 54); what lies behind the last index of a contraction is 0 or is
 // not looked at.
 
 // ---- shrink ---------------------------------------------------------------------------------------
 
-// A tile of 64 rows x RP ranks.  A thread owns 4 rows x RT ranks; the threads that cover the tile once form a k group, and
-// the k groups of the CTA share out the contraction index of every chunk of KC.  KMAJ: both operands
-// have the contraction index contiguous, a 128-bit load of each makes two packed multiply-adds per output (sums over even
-// and odd indices, added at the end); otherwise the ranks are contiguous and a packed multiply-add serves two of them.  The
-// CTAs of a cluster cut the contraction into contiguous ranges; k groups are added through shared memory, the cluster's
-// partial tiles through distributed shared memory, both in ascending order.
+// A tile of 64 rows x RP ranks.  The contraction index goes in slices of 16, dealt to the warps in turn; a warp covers all
+// 64 rows and RW (8 or 16) ranks of its slices, 4 rows x RW / 2 ranks per lane, and keeps them in a ring of its own, so that warps with
+// different slices never wait for one another (with a ring shared by the CTA and a barrier per 128 k: 59 us for 8192 x 4096
+// rows at rank 16, against 51 us).  Ranks beyond 16 take 2 or 4 warps per slice, which share its rows and a barrier.
+// The adapter's part of a slice is kept with the ranks contiguous: a packed multiply-add serves two of them.  KMAJ: in memory its
+// contraction index is contiguous, it is copied in pieces of 4 bytes.  The CTAs of a cluster cut the contraction into
+// contiguous ranges; slices are added through shared memory, the cluster's partial tiles through distributed shared
+// memory, both in ascending order.
 struct ShrinkParams {
     Groups g;
     const float* x;       // (rows, L)
@@ -189,33 +192,26 @@ struct ShrinkParams {
     int rows, L, rank;
 };
 
-template <int RP, bool KMAJ>
+template <int RP>
 struct ShrinkCfg {
-    static constexpr int RT = KMAJ ? 4 : 8;                  // ranks per thread
-    static constexpr int KC = KMAJ ? 64 : 128, LD = KC + 4, STAGES = KMAJ ? 3 : 2, X_FLOATS = TM * LD;
-    static constexpr int GROUP = 16 * RP / RT, KG = THREADS / GROUP;
-    static constexpr int MIN_CTAS = KMAJ ? 3 : 2;
-    static constexpr int RED_FLOATS = KG * TM * RP;
-    // row pitch of the adapter's part of a stage, and its floats (ranks behind the last one are read past a row's end)
-    __host__ __device__ static int pitch(int rank) { return KMAJ ? LD : (rank + 3) & ~3; }
-    __host__ __device__ static int w_floats(int rank) { return KMAJ ? RP * LD : KC * pitch(rank) + RP; }
-    static int smem_bytes(int rank)
-    {
-        const int ring = STAGES * (X_FLOATS + w_floats(rank));
-        return (ring > RED_FLOATS ? ring : RED_FLOATS) * 4;
-    }
+    static constexpr int KW = 16, LD = KW + 4, RW = RP < 16 ? RP : 16, RT = RW / 2;
+    static constexpr int RB = RP / RW, KS = THREADS / 32 / RB;                  // warps per slice, slices at a time
+    static constexpr int X_FLOATS = TM * LD, W_FLOATS = KW * RW, STAGE_FLOATS = X_FLOATS + RB * W_FLOATS;
+    static constexpr int STAGES = RB == 1 ? 2 : 3;
+    static constexpr int RED_FLOATS = KS * TM * RP, RING_FLOATS = KS * STAGES * STAGE_FLOATS;
+    static constexpr int SMEM_BYTES = (RING_FLOATS > RED_FLOATS ? RING_FLOATS : RED_FLOATS) * 4;
 };
 
 template <int RP, bool KMAJ, bool VEC>
-__global__ void __launch_bounds__(THREADS, (ShrinkCfg<RP, KMAJ>::MIN_CTAS)) shrink_kernel(const ShrinkParams p)
+__global__ void __launch_bounds__(THREADS, 2) shrink_kernel(const __grid_constant__ ShrinkParams p)
 {
-    using C = ShrinkCfg<RP, KMAJ>;
-    constexpr int KC = C::KC, LD = C::LD, STAGES = C::STAGES, RT = C::RT, GROUP = C::GROUP, KG = C::KG, QPG = KC / 4 / KG;
-    extern __shared__ __align__(16) float smem[];
+    using C = ShrinkCfg<RP>;
+    constexpr int KW = C::KW, LD = C::LD, STAGES = C::STAGES, RW = C::RW, RT = C::RT, RB = C::RB, KS = C::KS, Q = KW / 4;
+    extern __shared__ __align__(128) float smem[];
     __shared__ int row_s[TM];
     cg::cluster_group cluster = cg::this_cluster();
     const int S = static_cast<int>(cluster.num_blocks()), split = static_cast<int>(cluster.block_rank());
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, ks = warp / RB, wr = warp % RB;
     const int rb = blockIdx.y * RP;                                  // first rank of this block of ranks
     wait_for_previous();
     let_next_begin();
@@ -223,107 +219,123 @@ __global__ void __launch_bounds__(THREADS, (ShrinkCfg<RP, KMAJ>::MIN_CTAS)) shri
     if (!tile.valid) return;                                         // (the whole cluster)
     tile_row_numbers(p.g, tile, row_s);
     __syncthreads();
-    const int span = ((p.L + S - 1) / S + KC - 1) / KC * KC;
-    const int l0 = split * span, l1 = tile.adapter < 0 ? 0 : min(p.L, l0 + span);
-    const int chunks = l1 > l0 ? (l1 - l0 + KC - 1) / KC : 0;
-    const int pitch = C::pitch(p.rank), stage_floats = C::X_FLOATS + C::w_floats(p.rank);
+    constexpr int ROUND = KW * KS;                                   // contraction indices that the CTA takes at a time
+    const int span = ((p.L + S - 1) / S + ROUND - 1) / ROUND * ROUND;
+    const int l0 = split * span + ks * KW, l1 = tile.adapter < 0 ? 0 : min(p.L, split * span + span);
+    const int chunks = l1 > l0 ? (l1 - l0 + ROUND - 1) / ROUND : 0;  // of this warp
     const float* w = p.w + (tile.adapter < 0 ? 0ll : static_cast<long long>(tile.adapter) * p.rank * p.L);
-    const int wrows = min(RP, p.rank - rb);
+    const int r0 = rb + wr * RW, wn = min(RW, p.rank - r0);          // this warp's ranks (wn <= 0: none)
+    float* ring = smem + ks * STAGES * C::STAGE_FLOATS;
 
-    // VEC: this thread's places of a stage
-    constexpr int Q = KC / 4, XN = TM * Q / THREADS, WN = (RP * Q + THREADS - 1) / THREADS;
-    const int c4 = (tid % Q) * 4, xr = tid / Q;
+    // VEC: this lane's places of a stage
+    constexpr int XN = TM * Q / 32 / RB, WN = KMAJ ? 1 : RW * Q / 32;
+    const int c4 = (lane % Q) * 4, xr = wr * (TM / RB) + lane / Q;
+    constexpr int XSTEP = 32 / Q;
     int xat[XN], wat[WN];                      // (element offsets: int32 reaches every element of x and of one adapter)
+    bool wok[WN];
     if constexpr (VEC) {
 #pragma unroll
         for (int i = 0; i < XN; i++) {
-            const int r = row_s[xr + i * (THREADS / Q)];
+            const int r = row_s[xr + i * XSTEP];
             xat[i] = (r < 0 ? row_s[0] : r) * p.L + l0 + c4;
         }
 #pragma unroll
-        for (int i = 0; i < WN; i++) wat[i] = KMAJ ? (rb + min(xr + i * (THREADS / Q), wrows - 1)) * p.L + l0 + c4 : l0 * p.rank + tid * 4;
+        for (int i = 0; i < WN; i++) {
+            const int q = lane + 32 * i;
+            if constexpr (KMAJ) {
+                wat[0] = (r0 + lane / KW) * p.L + l0 + lane % KW;
+            } else {
+                wok[i] = (q % (RW / 4)) * 4 < wn;
+                wat[i] = (l0 + q / (RW / 4)) * p.rank + r0 + (q % (RW / 4)) * 4;
+            }
+        }
     }
     const auto issue = [&](int chunk) {
         if (chunk < chunks) {
-            float* xs = smem + (chunk % STAGES) * stage_floats;
-            float* ws = xs + C::X_FLOATS;
-            const int l = l0 + chunk * KC, kn = min(KC, l1 - l);
+            float* xs = ring + (chunk % STAGES) * C::STAGE_FLOATS;
+            float* ws = xs + C::X_FLOATS + wr * C::W_FLOATS;
+            const int at = chunk * ROUND, l = l0 + at, kn = min(KW, l1 - l);
             if constexpr (VEC) {
                 if (c4 < kn) {
 #pragma unroll
-                    for (int i = 0; i < XN; i++) copy16(xs + (xr + i * (THREADS / Q)) * LD + c4, p.x + xat[i] + chunk * KC);
-                    if constexpr (KMAJ) {
+                    for (int i = 0; i < XN; i++) copy16(xs + (xr + i * XSTEP) * LD + c4, p.x + xat[i] + at);
+                }
+                if constexpr (KMAJ) {
+                    if (lane % KW < kn) {
+                        const float* src = w + wat[0] + at;
+                        float* dst = ws + (lane % KW) * RW + lane / KW;
 #pragma unroll
-                        for (int i = 0; i < WN; i++)
-                            if (RP * Q >= THREADS || xr < RP) copy16(ws + (xr + i * (THREADS / Q)) * LD + c4, w + wat[i] + chunk * KC);
+                        for (int i = 0; i < RW * KW / 32; i++)
+                            if (lane / KW + i * (32 / KW) < wn) copy1(dst + i * (32 / KW), src + i * (32 / KW) * p.L, true);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < WN; i++) {
+                        const int q = lane + 32 * i;
+                        if (wok[i] && q / (RW / 4) < kn) copy16(ws + q * 4, w + wat[i] + at * p.rank);
                     }
                 }
-                if constexpr (!KMAJ) {
-                    // (all ranks of kn steps: one dense block)
-                    const int n4 = kn * p.rank / 4;
-                    const float* src = w + wat[0] + chunk * KC * p.rank;
-                    for (int q = tid; q < n4; q += THREADS, src += THREADS * 4) copy16(ws + q * 4, src);
-                }
             } else {
-                for (int q = tid; q < TM * KC; q += THREADS) {
-                    const int r = q / KC, c = q % KC;
+                for (int q = lane + 32 * wr; q < TM * KW; q += 32 * RB) {
+                    const int r = q / KW, c = q % KW;
                     const bool there = c < kn && row_s[r] >= 0;
                     copy1(xs + r * LD + c, there ? p.x + static_cast<long long>(row_s[r]) * p.L + l + c : p.x, there);
                 }
-                for (int q = tid; q < RP * KC; q += THREADS) {
-                    const int r = KMAJ ? q / KC : q % RP, c = KMAJ ? q % KC : q / RP;
-                    const bool there = c < kn && r < wrows;
-                    if (KMAJ || there || rb + r < pitch)
-                        copy1(KMAJ ? ws + r * LD + c : ws + c * pitch + rb + r,
-                              there ? w + (KMAJ ? static_cast<long long>(rb + r) * p.L + l + c : static_cast<long long>(l + c) * p.rank + rb + r) : p.w, there);
+                for (int q = lane; q < RW * KW; q += 32) {
+                    const int r = KMAJ ? q / KW : q % RW, c = KMAJ ? q % KW : q / RW;
+                    const bool there = c < kn && r < wn;
+                    copy1(ws + c * RW + r,
+                          there ? w + (KMAJ ? static_cast<long long>(r0 + r) * p.L + l + c : static_cast<long long>(l + c) * p.rank + r0 + r) : p.w, there);
                 }
             }
         }
         commit_copies();
     };
+    // the warps of one slice
+    const auto meet = [&]() {
+        if constexpr (RB == 1) __syncwarp();
+        else asm volatile("bar.sync %0, %1;" ::"r"(1 + ks), "n"(32 * RB) : "memory");
+    };
 
-    const int kg = tid / GROUP, t = tid % GROUP, rg = t % 16, cgp = t / 16;
-    float2 acc[4][4];                          // KMAJ: (even, odd) sums of four ranks; else four rank pairs
+    const int rg = lane % 16, cgp = lane / 16;
+    constexpr int NA = RT / 2;
+    float2 acc[4][NA];                         // [row][pair of ranks]
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) acc[i][j] = make_float2(0.f, 0.f);
+        for (int j = 0; j < NA; j++) acc[i][j] = make_float2(0.f, 0.f);
     for (int s = 0; s < STAGES - 1; s++) issue(s);
     for (int done = 0; done < chunks; done++) {
-        wait_copies<STAGES - 2>();
-        __syncthreads();
-        issue(done + STAGES - 1);
-        const float* xs = smem + (done % STAGES) * stage_floats;
-        const float* ws = xs + C::X_FLOATS + (KMAJ ? 0 : rb);
-        const int kn = min(KC, l1 - l0 - done * KC);
+        if constexpr (STAGES > 2) {
+            wait_copies<STAGES - 2>();
+            meet();
+            issue(done + STAGES - 1);
+        } else {
+            // (two stages: the other one was read in the previous step, by the same warp)
+            __syncwarp();
+            issue(done + 1);
+            wait_copies<1>();
+            __syncwarp();
+        }
+        const float* xs = ring + (done % STAGES) * C::STAGE_FLOATS;
+        const float* ws = xs + C::X_FLOATS + wr * C::W_FLOATS;
+        const int kn = min(KW, l1 - l0 - done * ROUND);
 #pragma unroll
-        for (int qq = 0; qq < QPG; qq++) {
-            const int k = (kg * QPG + qq) * 4;
+        for (int k = 0; k < KW; k += 4) {
             if (k >= kn) break;
             float4 xv[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) xv[i] = *reinterpret_cast<const float4*>(xs + (rg + 16 * i) * LD + k);
-            if constexpr (KMAJ) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const float4 wv = *reinterpret_cast<const float4*>(ws + (cgp + RP / 4 * j) * LD + k);
+            for (int kk = 0; kk < 4; kk++) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) acc[i][j] = __ffma2_rn(make_float2(xv[i].x, xv[i].y), make_float2(wv.x, wv.y), acc[i][j]);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) acc[i][j] = __ffma2_rn(make_float2(xv[i].z, xv[i].w), make_float2(wv.z, wv.w), acc[i][j]);
-                }
-            } else {
-#pragma unroll
-                for (int kk = 0; kk < 4; kk++) {
-                    const float4 w0 = *reinterpret_cast<const float4*>(ws + (k + kk) * pitch + cgp * 8);
-                    const float4 w1 = *reinterpret_cast<const float4*>(ws + (k + kk) * pitch + cgp * 8 + 4);
+                for (int j = 0; j < RT / 4; j++) {
+                    const float4 wv = *reinterpret_cast<const float4*>(ws + (k + kk) * RW + cgp * RT + 4 * j);
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const float xk = kk == 0 ? xv[i].x : kk == 1 ? xv[i].y : kk == 2 ? xv[i].z : xv[i].w;
-                        acc[i][0] = __ffma2_rn(make_float2(xk, xk), make_float2(w0.x, w0.y), acc[i][0]);
-                        acc[i][1] = __ffma2_rn(make_float2(xk, xk), make_float2(w0.z, w0.w), acc[i][1]);
-                        acc[i][2] = __ffma2_rn(make_float2(xk, xk), make_float2(w1.x, w1.y), acc[i][2]);
-                        acc[i][3] = __ffma2_rn(make_float2(xk, xk), make_float2(w1.z, w1.w), acc[i][3]);
+                        acc[i][2 * j] = __ffma2_rn(make_float2(xk, xk), make_float2(wv.x, wv.y), acc[i][2 * j]);
+                        acc[i][2 * j + 1] = __ffma2_rn(make_float2(xk, xk), make_float2(wv.z, wv.w), acc[i][2 * j + 1]);
                     }
                 }
             }
@@ -331,18 +343,17 @@ __global__ void __launch_bounds__(THREADS, (ShrinkCfg<RP, KMAJ>::MIN_CTAS)) shri
     }
     wait_copies<0>();
     __syncthreads();
-    // partial tiles [kg][row][rank]
+    // partial tiles [slice][row][rank]
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int j = 0; j < RT; j++)
-            smem[(kg * TM + rg + 16 * i) * RP + (KMAJ ? cgp + RP / 4 * j : cgp * 8 + j)] =
-                KMAJ ? acc[i][j % 4].x + acc[i][j % 4].y : (j & 1 ? acc[i][j / 2].y : acc[i][j / 2].x);
+            smem[(ks * TM + rg + 16 * i) * RP + wr * RW + cgp * RT + j] = j & 1 ? acc[i][j / 2].y : acc[i][j / 2].x;
     __syncthreads();
-    for (int e = tid; e < TM * RP && KG > 1; e += THREADS) {
+    for (int e = tid; e < TM * RP; e += THREADS) {
         float s = smem[e];
 #pragma unroll
-        for (int q = 1; q < KG; q++) s += smem[q * TM * RP + e];
+        for (int q = 1; q < KS; q++) s += smem[q * TM * RP + e];
         smem[e] = s;
     }
     const float scale = p.scale && tile.adapter >= 0 ? __ldg(p.scale + tile.adapter) : 1.f;
@@ -382,10 +393,10 @@ struct ExpandCfg {
 };
 
 template <int RC, bool RMAJ, bool VEC>
-__global__ void __launch_bounds__(THREADS, 3) expand_kernel(const ExpandParams p)
+__global__ void __launch_bounds__(THREADS, 3) expand_kernel(const __grid_constant__ ExpandParams p)
 {
     using C = ExpandCfg<RC>;
-    extern __shared__ __align__(16) float smem[];
+    extern __shared__ __align__(128) float smem[];
     __shared__ int row_s[TM];
     const Tile tile = tile_of(p.g, blockIdx.x, p.rows);
     if (p.wait_first) wait_for_previous();
@@ -405,20 +416,15 @@ __global__ void __launch_bounds__(THREADS, 3) expand_kernel(const ExpandParams p
     const int steps = (ct1 - ct0) * rchunks;
     const float* w = p.w + static_cast<long long>(with ? tile.adapter : 0) * p.rank * p.J;
 
-    int cat[8];                                            // VEC: element offsets of this lane's columns of its warp's rows
-    if constexpr (VEC) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int m = row_s[warp * 8 + i];
-            cat[i] = (m < 0 ? row_s[0] : m) * p.J + ct0 * EN + lane * 4;
-        }
-    }
     const auto issue_c = [&](int ct) {
         const int j0 = (ct0 + ct) * EN, jn = min(EN, p.J - j0);
         if constexpr (VEC) {
             if (lane * 4 < jn) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) copy16(cs + (warp * 8 + i) * EN + lane * 4, p.c + cat[i] + ct * EN);
+                for (int i = 0; i < 8; i++) {
+                    const int m = row_s[warp * 8 + i];       // (int32 offsets reach every element of c)
+                    copy16(cs + (warp * 8 + i) * EN + lane * 4, p.c + ((m < 0 ? row_s[0] : m) * p.J + j0 + lane * 4));
+                }
             }
         } else {
             for (int i = 0; i < 8; i++) {
@@ -565,11 +571,11 @@ struct OuterCfg {
 };
 
 template <int RP, bool VEC>
-__global__ void __launch_bounds__(THREADS, 2) outer_kernel(const OuterParams p)
+__global__ void __launch_bounds__(THREADS, 2) outer_kernel(const __grid_constant__ OuterParams p)
 {
     using C = OuterCfg<RP>;
     constexpr int MC = C::MC, CN = C::CN, STAGES = C::STAGES, RT = C::RT, GROUP = C::GROUP, MG = C::MG;
-    extern __shared__ __align__(16) float smem[];
+    extern __shared__ __align__(128) float smem[];
     cg::cluster_group cluster = cg::this_cluster();
     const int S = static_cast<int>(cluster.num_blocks()), split = static_cast<int>(cluster.block_rank());
     const int tid = threadIdx.x, e = blockIdx.y, rb = blockIdx.z * RP;
@@ -744,9 +750,9 @@ template <int RP, bool KMAJ>
 cudaError_t launch_shrink_t(cudaStream_t st, const ShrinkParams& p, int tiles, bool vec, bool early, int num_sms)
 {
     const int rblocks = (p.rank + RP - 1) / RP;
-    const int S = cluster_size(static_cast<long long>(tiles) * rblocks, p.L, 128, ShrinkCfg<RP, KMAJ>::MIN_CTAS, num_sms);
+    const int S = cluster_size(static_cast<long long>(tiles) * rblocks, p.L, 128, 2, num_sms);
     const dim3 grid(static_cast<unsigned int>(tiles) * S, rblocks, 1);
-    const int smem = ShrinkCfg<RP, KMAJ>::smem_bytes(p.rank);
+    const int smem = ShrinkCfg<RP>::SMEM_BYTES;
     return vec ? launch_cluster(st, shrink_kernel<RP, KMAJ, true>, grid, S, smem, early, p)
                : launch_cluster(st, shrink_kernel<RP, KMAJ, false>, grid, S, smem, early, p);
 }
@@ -776,10 +782,9 @@ cudaError_t allow_smem(K* kernel, int bytes) { return cudaFuncSetAttribute(kerne
 template <int RP, bool VEC>
 cudaError_t init_rank()
 {
-    const int most = RP == 64 ? MAX_RANK : RP;
     cudaError_t e;
-    if ((e = allow_smem(shrink_kernel<RP, true, VEC>, ShrinkCfg<RP, true>::smem_bytes(most))) != cudaSuccess) return e;
-    if ((e = allow_smem(shrink_kernel<RP, false, VEC>, ShrinkCfg<RP, false>::smem_bytes(most))) != cudaSuccess) return e;
+    if ((e = allow_smem(shrink_kernel<RP, true, VEC>, ShrinkCfg<RP>::SMEM_BYTES)) != cudaSuccess) return e;
+    if ((e = allow_smem(shrink_kernel<RP, false, VEC>, ShrinkCfg<RP>::SMEM_BYTES)) != cudaSuccess) return e;
     return allow_smem(outer_kernel<RP, VEC>, OuterCfg<RP>::SMEM_BYTES);
 }
 
@@ -805,8 +810,7 @@ cudaError_t init_vec()
 
 size_t groups_bytes(int rows, int adapters)
 {
-    return up256(sizeof(int) * static_cast<size_t>(rows)) + up256(sizeof(int) * (static_cast<size_t>(adapters) + 3)) +
-           3 * up256(sizeof(int) * static_cast<size_t>(tile_bound(rows, adapters)));
+    return up256(sizeof(int) * static_cast<size_t>(rows)) + up256(sizeof(int) * (static_cast<size_t>(adapters) + 2));
 }
 
 Groups groups_layout(void* mem, int rows, int adapters)
@@ -814,22 +818,16 @@ Groups groups_layout(void* mem, int rows, int adapters)
     Groups g;
     uint8_t* at = static_cast<uint8_t*>(mem);
     g.max_tiles = tile_bound(rows, adapters);
-    const size_t t = up256(sizeof(int) * static_cast<size_t>(g.max_tiles));
+    g.count = adapters;
     g.perm = reinterpret_cast<int*>(at);
-    at += up256(sizeof(int) * static_cast<size_t>(rows));
-    g.offset = reinterpret_cast<int*>(at);
-    g.n_tiles = g.offset + adapters + 2;
-    at += up256(sizeof(int) * (static_cast<size_t>(adapters) + 3));
-    g.tile_adapter = reinterpret_cast<int*>(at);
-    g.tile_first = reinterpret_cast<int*>(at + t);
-    g.tile_rows = reinterpret_cast<int*>(at + 2 * t);
+    g.offset = reinterpret_cast<int*>(at + up256(sizeof(int) * static_cast<size_t>(rows)));
     return g;
 }
 
 cudaError_t launch_group(cudaStream_t st, const Groups& g, const int* row_adapter, int rows, int adapters,
-                         unsigned int* ticket, unsigned int* status)
+                         unsigned int* status)
 {
-    group_kernel<<<adapters + 1, THREADS, 0, st>>>(g, row_adapter, rows, adapters, ticket, status);
+    group_kernel<<<adapters + 1, GROUP_THREADS, 0, st>>>(g, row_adapter, rows, adapters, status);
     return cudaGetLastError();
 }
 

@@ -17,27 +17,22 @@ struct Adapters {
 };
 
 // Rows grouped by adapter, in device memory: perm lists the rows adapter by adapter (ascending row index within
-// one), offset[e] .. offset[e + 1] is adapter e's range of it, entry `count` holds the rows without an adapter, and
-// tile i covers tile_rows[i] entries of perm from tile_first[i] on, all of adapter tile_adapter[i] (-1: none).
-// All pointers null: every row has adapter 0, in its own order.
+// one) and behind them the rows without one; offset[e] .. offset[e + 1] is adapter e's range of it, entries `count` and
+// `count` + 1 hold the range of the rows without an adapter.  perm null: every row has adapter 0, in its own order.
 struct Groups {
     int* perm = nullptr;
     int* offset = nullptr;        // count + 2 entries
-    int* tile_adapter = nullptr;
-    int* tile_first = nullptr;
-    int* tile_rows = nullptr;
-    int* n_tiles = nullptr;
-    int max_tiles = 0;            // launch bound: at least *n_tiles
+    int count = 0;                // adapters
+    int max_tiles = 0;            // launch bound: at least the number of tiles
 };
 
 // Bytes of device memory the grouping of `rows` rows over `adapters` adapters takes, and its layout inside `mem`.
 size_t groups_bytes(int rows, int adapters);
 Groups groups_layout(void* mem, int rows, int adapters);
 
-// Groups the rows.  `ticket` is a device word that is zero between launches.  An index outside [-1, adapters) counts
-// as -1 and records DEV_BAD_ADAPTER in *status.
+// Groups the rows.  An index outside [-1, adapters) counts as -1 and records DEV_BAD_ADAPTER in *status.
 cudaError_t launch_group(cudaStream_t st, const Groups& g, const int* row_adapter, int rows, int adapters,
-                         unsigned int* ticket, unsigned int* status);
+                         unsigned int* status);
 
 // `early`: the launch directly in front, on the same stream, is one of this file's and of the same call; the two then
 // overlap.  `wait_first`: it is the one that writes t or c.  `t_is_new`: it is the one that writes t (else dt, if any).

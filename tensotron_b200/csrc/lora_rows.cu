@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p)
     // is stored pair by pair, and a packed multiply-add serves two rows.
     constexpr bool PAIRS = MT > 8;
     constexpr int NA = PAIRS ? MT / 2 : MT, VALUES = WARPS * NR * MT;
-    extern __shared__ __align__(16) float rows_smem[];
+    extern __shared__ __align__(128) float rows_smem[];
     __shared__ int adapter_s[MT];
     __shared__ float scale_s[MT];
     cg::cluster_group cluster = cg::this_cluster();
