@@ -163,7 +163,8 @@ TT_API int tt_linear_bwd(tt_handle_t h, void* stream, const float* x, const floa
  * db (adapters, N, rank) are written, zero for adapters without rows; they are not accumulated.  Outputs must not
  * overlap inputs or each other, other than by the accumulation into y or dx.
  * The projection's products follow the handle's math mode; the adapters' are always strict FP32.  Every sum runs in an
- * order that depends on the shapes, the row_adapter values and the SM count only (no atomics on data).
+ * order that depends on the shapes, the row_adapter values, the alignment and the SM count only (no atomics on data).
+ * A forward call of up to 64 rows in strict FP32 (16 in the other modes) takes two launches, which read w once per 16 rows.
  * M may be 0; N and K are at least 1.  Rank up to TT_LORA_MAX_RANK and up to TT_LORA_MAX_ADAPTERS adapters (TT_ERR_UNSUPPORTED beyond).  The handle workspace
  * holds the grouping of the rows (about 4 * (M + adapters) bytes), t and dt (M * rank floats each) and, for a
  * backward call with an activation, g (M * N floats): tt_lora_workspace bytes, TT_ERR_WORKSPACE when it is smaller. */
@@ -215,7 +216,9 @@ TT_API int tt_clip_grad_norm(tt_handle_t h, void* stream, float* grads, long lon
  * The squares are summed in double precision in an order that depends on the sizes, the tensors' alignment and the SM
  * count only.  A NaN among the gradients makes the norm and the coefficient NaN (and so, when scaled, every
  * gradient); an infinite one makes the coefficient 0.  A tensor may have zero elements (its pointer is then not read);
- * an empty list has norm 0.  Pointers are 4-byte aligned.  Needs 136 KiB of the handle workspace. */
+ * an empty list has norm 0.  Pointers are 4-byte aligned; tensors that are scaled must not overlap one another.  Lists of
+ * up to 32768 elements in 1024 tensors take one launch, others two (more beyond 1024 tensors).  Needs 136 KiB of the handle
+ * workspace. */
 TT_API int tt_clip_grad_norm_list(tt_handle_t h, void* stream, int count, float* const* grads, const long long* sizes,
                                   float max_norm, float eps, int scale, float* norm_out, float* coef_out);
 
@@ -265,8 +268,8 @@ TT_API int tt_adam_step(tt_handle_t h, void* stream, float* p, const float* g, f
 /* tt_adam_step over a parameter list (Adam.Step of src/Tensotron/Optimizers.cs:144-193, which launches once per
  * tensor): p[i], g[i], m[i], v[i] of sizes[i] elements (host arrays, read during the call and not retained), `adv` and
  * the scalars as in tt_adam_step.  grad_scale: optional device float that multiplies every gradient first, the
- * coef_out of tt_clip_grad_norm_list: the clipped step then neither writes nor re-reads the gradients.  With `advance`
- * the step counter moves once per call, also for an empty list. */
+ * coef_out of tt_clip_grad_norm_list: the clipped step then does not write the gradients.  With `advance` the step counter
+ * moves once per call, also for an empty list.  The tensors must not overlap one another. */
 TT_API int tt_adam_step_list(tt_handle_t h, void* stream, int count, float* const* p, const float* const* g,
                              float* const* m, float* const* v, const long long* sizes, float* adv,
                              const float* grad_scale, float beta1, float beta2, float lr, float eps, float coupled_wd,

@@ -1257,7 +1257,7 @@ int lora_check(tt_handle_t h, const tt_lora_desc* lora, int M, int N, int K, int
         return fail(h, TT_ERR_UNSUPPORTED, "more adapters or a higher rank than the kernels take");
     if (!lora->a || !lora->b) return fail(h, TT_ERR_INVALID_ARG, "null device pointer");
     if (M > (1 << 30) || static_cast<long long>(M) * lora->rank > 0x7fffffffll || static_cast<long long>(M) * N > 0x7fffffffll ||
-        static_cast<long long>(M) * K > 0x7fffffffll || (N + 127) / 128 > 65535 || (K + 127) / 128 > 65535)
+        static_cast<long long>(M) * K > 0x7fffffffll || N > 65535 * 128 || K > 65535 * 128)
         return fail(h, TT_ERR_UNSUPPORTED, "more elements than int32 offsets reach");   // like every buffer of the reference
     return TT_OK;
 }

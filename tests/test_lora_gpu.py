@@ -60,6 +60,26 @@ def run_fwd(rt, d, kind, proj, want_t=True, offset=0):
     return y.get(), t.get() if want_t else None
 
 
+# Few rows: w cut over 4 and 8 CTAs along k, more outputs than one pass of the SMs takes (also odd ones), a k that does not
+# fit and goes to the tiles, one row more than that form takes
+FEW_ROWS = [(16, 64, 8192, 8, 3), (13, 100, 16384, 4, 3), (9, 24, 20000, 4, 2), (3, 40, 20000, 16, 5), (1, 8, 40000, 4, 2), (4, 10000, 128, 8, 3),
+            (2, 20011, 64, 6, 3), (5, 9001, 33, 3, 2), (64, 300, 260, 16, 9), (65, 300, 260, 16, 9), (33, 777, 1028, 128, 4), (48, 4096, 516, 2, 60)]
+
+
+@pytest.mark.parametrize("proj", [True, False])
+@pytest.mark.parametrize("shape", FEW_ROWS)
+def test_forward_of_few_rows(rt, shape, proj):
+    m, n, k, r, e = shape
+    kind = ["none", "relu", "tanh"][(m + n) % 3]
+    d = ref.inputs(m * 7 + r, m, n, k, r, e, "mixed")
+    y, t, ey, et = ref.forward(d["x"], d["w"] if proj else None, d["bias"], d["a"], d["b"], d["s"], d["idx"], kind, d["y"])
+    gy, gt = run_fwd(rt, d, kind, proj)
+    near(gt, t, et, "t")
+    near(gy, y, ey, "y")
+    again = run_fwd(rt, d, kind, proj)
+    assert np.array_equal(gy, again[0]) and np.array_equal(gt, again[1])
+
+
 # rows, n, k, rank, adapters: single tokens, few rows, one row more and less than a tile, odd sizes, ranks between the
 # kernels' widths and the highest, more adapters than rows, narrow and long contractions
 SHAPES = [(1, 64, 64, 4, 3), (1, 1, 1, 1, 1), (2, 5, 3, 2, 1), (5, 33, 17, 1, 2), (16, 256, 512, 16, 40), (17, 130, 260, 8, 4),
@@ -297,6 +317,7 @@ def test_refusals(rt):
     assert status(adapters=LoraAdapters(f(1, 129, 8), f(1, 6, 129))) == 3
     assert status(adapters=LoraAdapters(f(4097, 1, 1), f(4097, 6, 1))) == 3
     assert status(M=1 << 20, N=1 << 12) == 3                    # offsets beyond int32
+    assert status(M=0, N=2 ** 31 - 1) == 3 and status(M=0, K=2 ** 31 - 1) == 3
     tiny = TensorRuntime(0, 4096)
     with pytest.raises(TensotronGemmError) as err:
         tiny.LaunchLoraForward(**{**ok, "x": f(2000, 8), "y": f(2000, 6), "M": 2000})
