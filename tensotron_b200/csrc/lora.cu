@@ -192,11 +192,12 @@ struct ShrinkParams {
     int rows, L, rank;
 };
 
-template <int RP>
+template <int RP, bool KMAJ>
 struct ShrinkCfg {
     static constexpr int KW = 16, LD = KW + 4, RW = RP < 16 ? RP : 16, RT = RW / 2;
     static constexpr int RB = RP / RW, KS = THREADS / 32 / RB;                  // warps per slice, slices at a time
-    static constexpr int X_FLOATS = TM * LD, W_FLOATS = KW * RW, STAGE_FLOATS = X_FLOATS + RB * W_FLOATS;
+    // (rows of 16 ranks, 16 floats apart, would put the pieces of a K-major copy on two banks)
+    static constexpr int X_FLOATS = TM * LD, PITCH = KMAJ ? RW + 4 : RW, W_FLOATS = KW * PITCH, STAGE_FLOATS = X_FLOATS + RB * W_FLOATS;
     static constexpr int STAGES = RB == 1 ? 2 : 3;
     static constexpr int RED_FLOATS = KS * TM * RP, RING_FLOATS = KS * STAGES * STAGE_FLOATS;
     static constexpr int SMEM_BYTES = (RING_FLOATS > RED_FLOATS ? RING_FLOATS : RED_FLOATS) * 4;
@@ -205,7 +206,7 @@ struct ShrinkCfg {
 template <int RP, bool KMAJ, bool VEC>
 __global__ void __launch_bounds__(THREADS, 2) shrink_kernel(const __grid_constant__ ShrinkParams p)
 {
-    using C = ShrinkCfg<RP>;
+    using C = ShrinkCfg<RP, KMAJ>;
     constexpr int KW = C::KW, LD = C::LD, STAGES = C::STAGES, RW = C::RW, RT = C::RT, RB = C::RB, KS = C::KS, Q = KW / 4;
     extern __shared__ __align__(128) float smem[];
     __shared__ int row_s[TM];
@@ -263,7 +264,7 @@ __global__ void __launch_bounds__(THREADS, 2) shrink_kernel(const __grid_constan
                 if constexpr (KMAJ) {
                     if (lane % KW < kn) {
                         const float* src = w + wat[0] + at;
-                        float* dst = ws + (lane % KW) * RW + lane / KW;
+                        float* dst = ws + (lane % KW) * C::PITCH + lane / KW;
 #pragma unroll
                         for (int i = 0; i < RW * KW / 32; i++)
                             if (lane / KW + i * (32 / KW) < wn) copy1(dst + i * (32 / KW), src + i * (32 / KW) * p.L, true);
@@ -284,7 +285,7 @@ __global__ void __launch_bounds__(THREADS, 2) shrink_kernel(const __grid_constan
                 for (int q = lane; q < RW * KW; q += 32) {
                     const int r = KMAJ ? q / KW : q % RW, c = KMAJ ? q % KW : q / RW;
                     const bool there = c < kn && r < wn;
-                    copy1(ws + c * RW + r,
+                    copy1(ws + c * C::PITCH + r,
                           there ? w + (KMAJ ? static_cast<long long>(r0 + r) * p.L + l + c : static_cast<long long>(l + c) * p.rank + r0 + r) : p.w, there);
                 }
             }
@@ -330,7 +331,7 @@ __global__ void __launch_bounds__(THREADS, 2) shrink_kernel(const __grid_constan
             for (int kk = 0; kk < 4; kk++) {
 #pragma unroll
                 for (int j = 0; j < RT / 4; j++) {
-                    const float4 wv = *reinterpret_cast<const float4*>(ws + (k + kk) * RW + cgp * RT + 4 * j);
+                    const float4 wv = *reinterpret_cast<const float4*>(ws + (k + kk) * C::PITCH + cgp * RT + 4 * j);
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const float xk = kk == 0 ? xv[i].x : kk == 1 ? xv[i].y : kk == 2 ? xv[i].z : xv[i].w;
@@ -752,7 +753,7 @@ cudaError_t launch_shrink_t(cudaStream_t st, const ShrinkParams& p, int tiles, b
     const int rblocks = (p.rank + RP - 1) / RP;
     const int S = cluster_size(static_cast<long long>(tiles) * rblocks, p.L, 128, 2, num_sms);
     const dim3 grid(static_cast<unsigned int>(tiles) * S, rblocks, 1);
-    const int smem = ShrinkCfg<RP>::SMEM_BYTES;
+    const int smem = ShrinkCfg<RP, KMAJ>::SMEM_BYTES;
     return vec ? launch_cluster(st, shrink_kernel<RP, KMAJ, true>, grid, S, smem, early, p)
                : launch_cluster(st, shrink_kernel<RP, KMAJ, false>, grid, S, smem, early, p);
 }
@@ -783,8 +784,8 @@ template <int RP, bool VEC>
 cudaError_t init_rank()
 {
     cudaError_t e;
-    if ((e = allow_smem(shrink_kernel<RP, true, VEC>, ShrinkCfg<RP>::SMEM_BYTES)) != cudaSuccess) return e;
-    if ((e = allow_smem(shrink_kernel<RP, false, VEC>, ShrinkCfg<RP>::SMEM_BYTES)) != cudaSuccess) return e;
+    if ((e = allow_smem(shrink_kernel<RP, true, VEC>, ShrinkCfg<RP, true>::SMEM_BYTES)) != cudaSuccess) return e;
+    if ((e = allow_smem(shrink_kernel<RP, false, VEC>, ShrinkCfg<RP, false>::SMEM_BYTES)) != cudaSuccess) return e;
     return allow_smem(outer_kernel<RP, VEC>, OuterCfg<RP>::SMEM_BYTES);
 }
 
