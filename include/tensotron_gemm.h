@@ -164,7 +164,7 @@ TT_API int tt_linear_bwd(tt_handle_t h, void* stream, const float* x, const floa
  * overlap inputs or each other, other than by the accumulation into y or dx.
  * The projection's products follow the handle's math mode; the adapters' are always strict FP32.  Every sum runs in an
  * order that depends on the shapes, the row_adapter values, the alignment and the SM count only (no atomics on data).
- * A forward call of up to 64 rows in strict FP32 (16 in the other modes) takes two launches, which read w once per 16 rows.
+ * A backward call of a small layer without dw and dbias takes one launch.  A forward call of up to 64 rows in strict FP32 (16 in the other modes) takes two launches, which read w once per 16 rows.
  * M may be 0; N and K are at least 1.  Rank up to TT_LORA_MAX_RANK and up to TT_LORA_MAX_ADAPTERS adapters (TT_ERR_UNSUPPORTED beyond).  The handle workspace
  * holds the grouping of the rows (about 4 * (M + adapters) bytes), t and dt (M * rank floats each) and, for a
  * backward call with an activation, g (M * N floats): tt_lora_workspace bytes, TT_ERR_WORKSPACE when it is smaller. */

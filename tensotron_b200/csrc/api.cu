@@ -824,7 +824,7 @@ cudaError_t init_kernels()
                                                cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
     if (!g_generic_cluster16) cudaGetLastError();
     if (mlp_step::init_device() != 0) return cudaErrorUnknown;
-    if ((e = lora::init_tiled()) != cudaSuccess || (e = lora::init_rows()) != cudaSuccess) return e;
+    if ((e = lora::init_tiled()) != cudaSuccess || (e = lora::init_rows()) != cudaSuccess || (e = lora::init_small()) != cudaSuccess) return e;
     if ((e = cudaFuncSetAttribute(skinny::skinny_n_stream_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                   skinny::stream::Cfg<4>::SMEM_BYTES)) != cudaSuccess) return e;
     if ((e = cudaFuncSetAttribute(skinny::skinny_n_stream_kernel<8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -1351,6 +1351,12 @@ TT_API int tt_lora_bwd(tt_handle_t h, void* stream, const tt_lora_desc* lora, co
         return TT_OK;
     }
     const lora::Adapters ad{lora->a, lora->b, lora->scale, lora->adapters, lora->rank};
+    if (h->variant == 0 && !dw && !dbias && (t || !db) && lora::small_fits(M, N, K, lora->rank, lora->adapters)) {
+        e = lora::launch_bwd_small(st, ad, row_adapter, x, w, y, dy, t, dx, da, db, M, N, K, act, h->status);
+        if (e != cudaSuccess) return cuda_fail(h, e, "small adapter backward launch");
+        if (dx || da || db) h->stats.launches++;
+        return TT_OK;
+    }
     // g = dy * act'(y) and the bias gradient
     const float* grad = dy;
     if (act != TT_ACT_NONE || dbias) {

@@ -60,7 +60,15 @@ constexpr int MAX_ROWS_SMEM = 224 * 1024;
 cudaError_t launch_rows(cudaStream_t st, const Adapters& ad, const int* row_adapter, const float* x, const float* w,
                         const float* bias, float* y, float* t, int M, int N, int K, int act, unsigned int* status, int num_sms,
                         bool* taken);
+// The backward pass of a small layer's adapters in one launch (lora_small.cu): dx, da and db may each be null, t is given
+// when db is.  small_fits: whether the shape is one it holds.
+bool small_fits(int M, int N, int K, int rank, int count);
+cudaError_t launch_bwd_small(cudaStream_t st, const Adapters& ad, const int* row_adapter, const float* x, const float* w,
+                             const float* y, const float* dy, const float* t, float* dx, float* da, float* db, int M, int N, int K,
+                             int act, unsigned int* status);
+
 // Kernel attributes, once per context (called from tt_create).
+cudaError_t init_small();
 cudaError_t init_tiled();
 cudaError_t init_rows();
 

@@ -126,9 +126,40 @@ def test_backward(rt, shape, proj, mix):
         d["y"] = np.tanh(d["y"])
     t = ref.forward(d["x"], None, None, d["a"], d["b"], d["s"], d["idx"], kind, d["y"])[1].astype(np.float32)
     want = ref.backward(d["x"], d["w"] if proj else None, d["a"], d["b"], d["s"], d["idx"], kind, d["y"], d["dy"], t, d["dx"])
-    got = run_bwd(rt, d, kind, proj, t)
+    for base in ([True, False] if proj else [False]):        # (without the projection's gradients small layers take one launch)
+        got = run_bwd(rt, d, kind, proj, t, base)
+        for name, v in got.items():
+            near(v, *want[name], name)
+
+
+# the one-launch form's limits (rows, outputs, rows x N, rows x rank, rank, adapters, adapters x N x rank, adapters x rank,
+# rows x N x K), and one beyond each
+SMALL = [(64, 64, 128, 4, 1), (256, 32, 256, 16, 2), (256, 32, 255, 8, 16), (32, 256, 256, 2, 16), (33, 248, 33, 5, 6), (1, 256, 1000, 16, 2), (7, 200, 299, 3, 13),
+         (256, 1, 31, 8, 3), (257, 8, 16, 4, 2), (20, 257, 16, 4, 2), (64, 129, 64, 4, 2), (64, 64, 64, 17, 2), (32, 32, 64, 4, 17), (8, 256, 16, 11, 3), (8, 16, 16, 13, 10),
+         (64, 64, 513, 4, 2)]
+
+
+@pytest.mark.parametrize("mix", ["mixed", "one", "none"])
+@pytest.mark.parametrize("proj", [True, False])
+@pytest.mark.parametrize("shape", SMALL)
+def test_backward_of_small_layers(rt, shape, proj, mix):
+    m, n, k, r, e = shape
+    kind = ["none", "relu", "tanh"][(n + k) % 3]
+    d = ref.inputs(m + 3 * k, m, n, k, r, e, mix)
+    if kind == "tanh":
+        d["y"] = np.tanh(d["y"])
+    t = ref.forward(d["x"], None, None, d["a"], d["b"], d["s"], d["idx"], kind, d["y"])[1].astype(np.float32)
+    want = ref.backward(d["x"], d["w"] if proj else None, d["a"], d["b"], d["s"], d["idx"], kind, d["y"], d["dy"], t, d["dx"])
+    rt.ResetCounters()
+    got = run_bwd(rt, d, kind, proj, t, base=False)
+    if not proj and mix == "mixed":
+        small = (m <= 256 and n <= 256 and r <= 16 and e <= 16 and m * n <= 8192 and m * r <= 4096 and e * n * r <= 8192 and
+                 e * r <= 128 and m * n * k <= 1 << 21)
+        assert (rt.Stats()["launches"] == 1) == small
     for name, v in got.items():
         near(v, *want[name], name)
+    again = run_bwd(rt, d, kind, proj, t, base=False)
+    assert all(np.array_equal(got[f], again[f]) for f in got)
 
 
 @pytest.mark.parametrize("offset", [1, 2, 3])
@@ -200,6 +231,15 @@ def test_bad_indices_are_reported_and_never_used(rt):
     near(oy.get(), y, ey, "y")
     near(ot.get(), t, et, "t")
     rt.Check()                                      # the report was taken back
+    want = ref.backward(d["x"], d["w"], d["a"], d["b"], d["s"], d["idx"], "none", d["y"], d["dy"], t)
+    for part in (dict(da=Out((3, 4, 48)), db=Out((3, 32, 4))), dict(dx=Out((80, 48)), dw=Out((32, 48)))):     # in one launch, and in several
+        rt.LaunchLoraBackward(ad, dev(bad), dev(d["x"]), dev(d["w"]), None, dev(d["dy"]), dev(t.astype(np.float32)),
+                              *[part[f].t if f in part else None for f in ("dx", "dw", "dbias", "da", "db")], 80, 32, 48)
+        with pytest.raises(TensotronGemmError) as err:
+            rt.Check()
+        assert err.value.status == 8
+        for name, v in part.items():
+            near(v.get(), *want[name], name)
 
 
 def test_not_finite_values_stay_with_their_rows_and_adapters(rt):
