@@ -357,7 +357,8 @@ TT_API int tt_check(tt_handle_t h, void* stream);
  *   through a thread-block cluster,
  * 9 FFMA kernel with 128x128 tiles and stream-K work distribution,
  * 10 automatic, but tall products with N <= 16 keep the K-cut streaming kernel instead of the
- *   TMA-fed one. */
+ *   TMA-fed one.
+ * Any variant but 0 also keeps tt_lora_fwd and tt_lora_bwd on their tiled kernels. */
 TT_API int tt_set_variant(tt_handle_t h, int variant);
 
 /* ---- Data-parallel gradient exchange over peer memory ---------------------------------

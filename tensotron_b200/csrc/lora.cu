@@ -6,7 +6,8 @@
 //
 // Rows are grouped by adapter first (group_kernel), so that a tile of 64 rows meets one adapter: its A and B are then
 // read once per tile from L2, and the four products become three tiled kernels:
-//     shrink_kernel   (rows x L) . (L x rank): a long contraction into a narrow output
+//     shrink_kernel   (rows x L) . (L x rank): a long contraction into a narrow output; 8192 x 4096 at rank 16: 41-49 us for
+//                     134 MB and 1.07 GFLOP (20.5 and 14.5 us at their rates)
 //     expand_kernel   (rows x rank) . (rank x J), added to what the output holds
 //     outer_kernel    (rank x rows) . (rows x C): contracts over the rows of one adapter
 #include "lora.h"
@@ -45,7 +46,8 @@ __device__ __forceinline__ void finish()
 
 // One CTA per group (adapters 0 .. count-1, then the rows without one).  A CTA counts the rows of all lower groups and,
 // warp by warp over contiguous row ranges, its own; the range counts give every warp its place, and a second walk
-// writes the row indices.  No atomics: ascending row order within a group, whatever the timing.
+// writes the row indices.  No atomics: ascending row order within a group, whatever the timing.  Bound by latency: 8192 rows,
+// 8 adapters 4.6 us, 333 rows 3.1.
 __global__ void __launch_bounds__(GROUP_THREADS)
 group_kernel(Groups g, const int* __restrict__ row_adapter, int rows, int count, unsigned int* status)
 {
@@ -375,6 +377,7 @@ __global__ void __launch_bounds__(THREADS, 2) shrink_kernel(const __grid_constan
 // write of c: a step (up to RC ranks of one column tile) asks for its part of c and for the adapter's ranks of the next
 // step, then computes, then adds c, which the same thread asked for and stores, so that c takes one buffer and no
 // barrier.  The rows' t are read once per CTA and kept rank by rank: a packed multiply-add takes two rows.
+// 8192 x 4096 at rank 16: 53 us for 268 MB (41 us at the copy rate); what it waits for is shared memory at 24 warps per SM.
 struct ExpandParams {
     Groups g;
     const float* t;       // (rows, rank)
@@ -547,7 +550,8 @@ __global__ void __launch_bounds__(THREADS, 3) expand_kernel(const __grid_constan
 // columns, a packed multiply-add serves two ranks; the 32 RP / RT threads that cover the tile once form a row group, and the
 // row groups of the CTA share out the rows of every chunk of 64.  The CTAs of a cluster cut the adapter's rows into
 // contiguous ranges.  Joins as in shrink_kernel.  Two jobs in one grid: dA (rank, K) from dt and x, dB (N, rank) from t
-// and g.
+// and g.  8192 rows, both of 4096 columns, rank 16: 70 us for 268 MB and 2.1 GFLOP (41 and 29 us at their rates), half of the
+// issue slots busy.
 struct OuterJob {
     const float* small;   // (rows, rank)
     const float* big;     // (rows, C)

@@ -8,6 +8,9 @@
 // shared memory in pairs of rows, where one 128-bit load feeds 4 NR multiply-adds (2 NR packed ones).  NR x MT sums per lane are added over the lanes by a
 // transposing tree (NR x MT shuffles in all).  Where x does not fit, or where cutting N alone leaves SMs idle, the CTAs of
 // a cluster cut k, and their sums are added through distributed shared memory in rank order.
+// 4096 -> 4096, rank 16, per call: one row 24 us, 16 rows with an adapter each 28.7, 32 rows 47, 64 rows 86 (tiled form: 136, 146, 151,
+// 155).  One row is bound by its 67 MB (10.3 us at the copy rate; a bare stream by the same copies takes 14.4) and about 4 us
+// in front of and behind it, 64 rows by multiply-adds (28.9 us at the peak) and w coming from L2 four times.
 #include "lora.h"
 
 #include <cooperative_groups.h>

@@ -85,7 +85,7 @@ def test_forward_of_few_rows(rt, shape, proj):
 SHAPES = [(1, 64, 64, 4, 3), (1, 1, 1, 1, 1), (2, 5, 3, 2, 1), (5, 33, 17, 1, 2), (16, 256, 512, 16, 40), (17, 130, 260, 8, 4),
           (63, 64, 128, 4, 1), (65, 127, 129, 5, 3), (64, 64, 128, 4, 1), (130, 257, 100, 7, 5), (333, 517, 1000, 6, 5),
           (200, 128, 256, 64, 3), (100, 130, 70, 100, 4), (96, 132, 64, 128, 2), (300, 96, 4096, 16, 40), (700, 512, 36, 33, 7),
-          (1030, 36, 516, 12, 200)]
+          (1030, 36, 516, 12, 200), (700, 36, 40, 3, 600), (300, 16, 24, 2, 4096)]
 
 
 @pytest.mark.parametrize("mix", ["mixed", "one", "sorted", "last", "none"])
@@ -242,10 +242,12 @@ def test_bad_indices_are_reported_and_never_used(rt):
             near(v.get(), *want[name], name)
 
 
-def test_not_finite_values_stay_with_their_rows_and_adapters(rt):
+@pytest.mark.parametrize("m,n,k", [(150, 70, 90), (60, 70, 90), (14, 33, 50)])
+def test_not_finite_values_stay_with_their_rows_and_adapters(rt, m, n, k):
     """A NaN in one adapter reaches its own rows and gradients only; an infinite row its own outputs and its adapter's
     gradients only; rows without an adapter meet none of it."""
-    d = ref.inputs(9, 150, 70, 90, 6, 4, "mixed")
+    d = ref.inputs(9, m, n, k, 6, 4, "mixed")
+    d["idx"][:4] = [2, 1, -1, 0]
     d["a"][1, 2, 3] = np.nan
     d["b"][1, 4, 2] = np.nan
     row = int(np.nonzero(d["idx"] == 2)[0][0])
