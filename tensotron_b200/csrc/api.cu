@@ -824,7 +824,9 @@ cudaError_t init_kernels()
                                                cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
     if (!g_generic_cluster16) cudaGetLastError();
     if (mlp_step::init_device() != 0) return cudaErrorUnknown;
-    if ((e = lora::init_tiled()) != cudaSuccess || (e = lora::init_rows()) != cudaSuccess || (e = lora::init_small()) != cudaSuccess) return e;
+    if ((e = lora::init_tiled()) != cudaSuccess || (e = lora::init_rows()) != cudaSuccess || (e = lora::init_small()) != cudaSuccess ||
+        (e = lists::init_lists()) != cudaSuccess)
+        return e;
     if ((e = cudaFuncSetAttribute(skinny::skinny_n_stream_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                   skinny::stream::Cfg<4>::SMEM_BYTES)) != cudaSuccess) return e;
     if ((e = cudaFuncSetAttribute(skinny::skinny_n_stream_kernel<8>, cudaFuncAttributeMaxDynamicSharedMemorySize,

@@ -838,7 +838,10 @@ cudaError_t launch_group(cudaStream_t st, const Groups& g, const int* row_adapte
 
 cudaError_t init_tiled()
 {
-    const cudaError_t e = init_vec<true>();
+    cudaFuncAttributes attr;                 // (asking for them loads the kernel: a first call may be inside a capture)
+    cudaError_t e = cudaFuncGetAttributes(&attr, group_kernel);
+    if (e != cudaSuccess) return e;
+    e = init_vec<true>();
     return e != cudaSuccess ? e : init_vec<false>();
 }
 

@@ -388,6 +388,10 @@ cudaError_t launch_rows_v(int mt, int nr, cudaStream_t st, const RowsParams& p, 
 
 cudaError_t init_rows()
 {
+    cudaFuncAttributes attr;                 // (loads the kernels that need no attribute, as for the others)
+    cudaError_t loaded = cudaFuncGetAttributes(&attr, rows_down_kernel<true>);
+    if (loaded == cudaSuccess) loaded = cudaFuncGetAttributes(&attr, rows_down_kernel<false>);
+    if (loaded != cudaSuccess) return loaded;
     const RowsParams none = {};
     for (int mt = 4; mt <= 16; mt *= 2) {
         for (int nr = 1; nr <= 8; nr++) {

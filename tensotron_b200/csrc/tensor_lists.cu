@@ -488,5 +488,32 @@ cudaError_t launch_adam(cudaStream_t st, int count, float* const* p, const float
     return adam_cap<ADAM_CAP>(st, count, p, g, m, v, sizes, a, num_sms, launches);
 }
 
+namespace {
+template <int CAP>
+cudaError_t load_norm()
+{
+    cudaFuncAttributes attr;
+    cudaError_t e = cudaFuncGetAttributes(&attr, norm_kernel<CAP>);
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, scale_kernel<CAP>);
+    return e != cudaSuccess ? e : cudaFuncGetAttributes(&attr, clip_small_kernel<CAP>);
+}
+
+template <int CAP>
+cudaError_t load_adam()
+{
+    cudaFuncAttributes attr;
+    return cudaFuncGetAttributes(&attr, adam_kernel<CAP>);
+}
+}  // namespace
+
+cudaError_t init_lists()
+{
+    cudaError_t e;
+    if ((e = load_norm<SMALL_CAP>()) != cudaSuccess || (e = load_norm<MID_CAP>()) != cudaSuccess || (e = load_norm<NORM_CAP>()) != cudaSuccess ||
+        (e = load_adam<SMALL_CAP>()) != cudaSuccess || (e = load_adam<MID_CAP>()) != cudaSuccess)
+        return e;
+    return load_adam<ADAM_CAP>();
+}
+
 }  // namespace lists
 }  // namespace tt

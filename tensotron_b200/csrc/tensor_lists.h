@@ -23,5 +23,8 @@ cudaError_t launch_adam(cudaStream_t st, int count, float* const* p, const float
                         float lr, float eps, float cwd, float dfac, bool advance, unsigned int* ticket, int num_sms,
                         long long* launches);
 
+// Loads the kernels, once per context (called from tt_create), so that a first call may be inside a capture.
+cudaError_t init_lists();
+
 }  // namespace lists
 }  // namespace tt

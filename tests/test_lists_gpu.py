@@ -240,3 +240,44 @@ def test_refusals(rt):
         tiny.LaunchClipGradNormList([t], 1.0)
     assert err.value.status == 4
     tiny.Dispose()
+
+
+FIRST_CALL = """
+import torch
+from tensotron_b200.runtime import LoraAdapters, TensorList, TensorRuntime
+rt = TensorRuntime(0)
+f = lambda *s: torch.ones(s, device="cuda")
+lists = [TensorList([f(40000), f(3)]) for _ in range(4)]
+adv, coef = torch.zeros(3, device="cuda"), torch.zeros(1, device="cuda")
+ad = LoraAdapters(f(2, 4, 64), f(2, 48, 4))
+rows = []
+for m in (3, 100):
+    idx = torch.arange(m, device="cuda", dtype=torch.int32) % 3 - 1
+    rows.append((m, idx, f(m, 64), f(48, 64), f(m, 48), f(m, 4), f(m, 64), f(2, 4, 64), f(2, 48, 4), f(48, 64)))
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    rt.LaunchClipGradNormList(lists[1], 1.0, coef_out=coef, scale=False)
+    rt.LaunchAdamList(*lists, adv, grad_scale=coef)
+    rt.LaunchClipGradNormList(lists[1], 100.0)
+    for m, idx, x, w, y, t, dx, da, db, dw in rows:
+        rt.LaunchLoraForward(ad, idx, x, w, None, y, t, m, 48, 64)
+        rt.LaunchLoraBackward(ad, idx, x, w, None, y, t, dx, None, None, da, db, m, 48, 64)
+        rt.LaunchLoraBackward(ad, idx, x, w, None, y, t, dx, dw, None, da, db, m, 48, 64)
+graph.replay()
+rt.Check()
+assert adv[0].item() == 1 and abs(coef.item() - 40003 ** -0.5) < 1e-6
+for m, idx, x, w, y, t, *_ in rows:
+    has = (idx >= 0).float()
+    assert torch.equal(t, (64 * has)[:, None].expand(m, 4)) and torch.equal(y, (64 + 256 * has)[:, None].expand(m, 48))
+print("captured first")
+"""
+
+
+def test_a_first_call_may_be_inside_a_capture(gemm_lib):
+    import os
+    import subprocess
+    import sys
+    from conftest import ROOT
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL], cwd=ROOT, env=dict(os.environ, PYTHONPATH=ROOT), capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured first" in r.stdout, r.stdout + r.stderr
