@@ -470,3 +470,37 @@ def test_adapter_training_step_end_to_end(rt):
         clear = np.abs(g) > 1e-3 * np.abs(g).max()
         assert clear.mean() > 0.5
         np.testing.assert_allclose(h(got)[clear], q[clear], atol=1e-5)
+
+
+def test_offsets_close_to_int32(rt):
+    """x and dx of almost 2^31 elements: the last rows' offsets only just fit an int32."""
+    m, n, k, r, e = 524287, 8, 4096, 2, 3
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    f = lambda *s: torch.randn(s, generator=gen, device="cuda")      # noqa: E731
+    x, dx, dy, a, b = f(m, k), f(m, k), f(m, n), f(e, r, k) / 64, f(e, n, r)
+    idx = torch.randint(-1, e, (m,), generator=gen, device="cuda").to(torch.int32)
+    ad = LoraAdapters(a, b)
+    t, y, da, dx0 = torch.empty((m, r), device="cuda"), torch.zeros((m, n), device="cuda"), torch.empty_like(a), dx[-300:].clone()
+    rt.LaunchLoraForward(ad, idx, x, None, None, y, t, m, n, k)
+    rt.LaunchLoraBackward(ad, idx, x, None, None, dy, None, dx, None, None, da, None, m, n, k)
+    rt.Check()
+    last = slice(m - 300, m)
+    h = lambda v: v.double().cpu().numpy()       # noqa: E731
+    args = [h(x[last]), None, None, h(a), h(b), np.ones(e), idx[last].cpu().numpy(), "none", np.zeros((300, n))]
+    wy, wt, ey, et = ref.forward(*args)
+    near(h(y[last]), wy, ey, "y")
+    near(h(t[last]), wt, et, "t")
+    want = ref.backward(args[0], None, h(a), h(b), np.ones(e), args[6], "none", np.zeros((300, n)), h(dy[last]), wt, h(dx0))
+    near(h(dx[last]), *want["dx"], "dx")
+    # dA over all rows: the same products added in 64 bits, against (count + 32) roundings of their absolute sum
+    sums, mass = torch.zeros((e, r, k), dtype=torch.float64, device="cuda"), torch.zeros((e, r, k), dtype=torch.float64, device="cuda")
+    for at in range(0, m, 32768):
+        rows = slice(at, min(m, at + 32768))
+        for i in range(e):
+            on = (idx[rows] == i).double()[:, None]
+            dt = (dy[rows].double() @ b[i].double()) * on
+            sums[i] += dt.T @ x[rows].double()
+            mass[i] += ((dy[rows].double().abs() @ b[i].double().abs()) * on).T @ x[rows].double().abs()
+    near(h(da), h(sums), (m + 32) * ref.U * h(mass), "da")
+    # (that bound is loose at this count: the error of a sum of random signs grows with the root of it)
+    assert float((da - sums).norm() / sums.norm()) < m ** 0.5 * ref.U
